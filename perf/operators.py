@@ -166,7 +166,8 @@ def run(state):
         scale = _type(state["scale"])
         if state["kind"] == "quantize":
             return ops_q4.dequantize(ops_q4.quantize(state["w"], group=state["group"], zeros=state["zeros"], scale_dtype=scale), _type(state["out"]))
-        w = ops_q4.Q4Weight(state["data"], state["n"], state["k"], group=state["group"], zeros=state["zeros"], scale_dtype=scale)
+        w = ops_q4.Q4Weight(state["data"], state["n"], state["k"], group=state["group"], zeros=state["zeros"], scale_dtype=scale,
+                            at_rest=True)                # a model's weights were there long before the call
         if state["kind"] == "linear":
             return ops_q4.gemm_q4(state["x"], w, _type(state["out"]))
         return ops_q4.gemm_q4(state["x"], w, gated=("swish_clamped", LIMIT, ALPHA) if state["act"] == "swish_clamped" else state["act"])

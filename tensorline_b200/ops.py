@@ -183,6 +183,9 @@ STATUS_ROLES = {1: "tcgen05 product: the copy thread waited for a free stage", 2
                 63: "matrix memory's outputs: the MMA warp waited for a stage", 64: "matrix memory's outputs: the workers waited for Q K",
                 65: "matrix memory's outputs: the workers waited for a sum", 66: "matrix memory's end states: the MMA warp waited for a free accumulator",
                 67: "matrix memory's outputs: the MMA warp waited for free accumulators",
+                71: "4-bit product: the copy thread waited for a free stage", 72: "4-bit product: the MMA warp waited for tokens or unpacked weights",
+                73: "4-bit product: the MMA warp waited for a free accumulator", 74: "4-bit product: the unpacking waited for weights or for room",
+                75: "4-bit product: the sums waited for weights or an accumulator",
                 20: "decode attention: a wait for a stage of keys and values"}
 
 

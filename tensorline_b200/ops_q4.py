@@ -1,0 +1,244 @@
+"""Weights of 4 bits: making them, and products with them (`csrc/gemm_q4.cu`, `csrc/quantize_q4.cu`).
+
+    w[n, k] = scale[n, k // group] * (code[n, k] - zero[n, k // group])
+
+codes and zeros are whole numbers 0..15 (zero = 8 where a matrix has none), scales bfloat16 or float32, a group is 32, 64 or 128 values along k.
+A matrix takes half a byte a value and its scales: 0.52 bytes in groups of 128 with bfloat16 scales and no zeros.
+
+    w = quantize(matrix)                          # or pack(codes, scales, zeros), for weights that were quantized elsewhere
+    y = gemm_q4(x, w)                             # x [T, K] bfloat16, y [T, N]
+    m = gemm_q4(x, gate_up, gated="silu")         # silu(gate) * up, where gate and up rows alternate in blocks of 64
+    matrix = dequantize(w)
+
+Launches go to the current stream of the tensors' device.  As with every matrix of this package, K is a multiple of 8.
+"""
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from . import ops
+from .csrc.build import load_library
+from .ops import KernelError, _check, _stream, device_status
+
+_P, _I, _F, _L = ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_longlong
+
+SOURCES = ["gemm_q4.cu", "quantize_q4.cu"]
+_SIGNATURES = {
+    "tl_q4_block_bytes": [_I, _I, _I],
+    "tl_gemm_q4": [_P, _L, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _I, _F, _F, _I, _P, _P],
+    "tl_quantize_q4": [_P, _I, _P, _I, _I, _I, _I, _I, _P],
+    "tl_dequantize_q4": [_P, _P, _I, _I, _I, _I, _I, _I, _P],
+}
+GROUPS = (32, 64, 128)
+ROWS = K_BLOCK = 128                                      # of a stored block
+CODE_BYTES = ROWS * K_BLOCK // 2
+_lib = None
+
+
+def lib():
+    global _lib
+    if _lib is None:
+        l = load_library("tl_q4", SOURCES)
+        for name, sig in _SIGNATURES.items():
+            fn = getattr(l, name)
+            fn.argtypes = sig
+            fn.restype = ctypes.c_int
+        _lib = l
+    return _lib
+
+
+def block_bytes(group: int, scale_dtype: torch.dtype, zeros: bool) -> int:
+    """Bytes of a stored block of 128 rows and 128 k: codes, scales, zeros."""
+    if group not in GROUPS:
+        raise KernelError(f"4-bit weights come in groups of {GROUPS} values, not {group}")
+    if scale_dtype is not torch.bfloat16 and scale_dtype is not torch.float32:
+        raise KernelError(f"scales of 4-bit weights are bfloat16 or float32, not {scale_dtype}")
+    return CODE_BYTES + K_BLOCK // group * ROWS * (scale_dtype.itemsize + (1 if zeros else 0))
+
+
+class Q4Weight:
+    """A matrix [n, k] of 4-bit weights in its stored form: `data` uint8 [ceil(n / 128), ceil(k / 128), block_bytes(..)], a block holding
+
+        codes   [4: k / 32][128: row][4: k / 8 % 4] words of 32 bits; k % 8 = 4 p + 2 q + h is at bit 16 h + 8 p + 4 q of its word
+        scales  [128 / group][128: row] of `scale_dtype`
+        zeros   [128 / group][128: row] uint8, if `zeros`
+
+    (what is stored behind row n and column k is not used).  `at_rest`: the program promises that no kernel which may still be running
+    when a product is launched writes `data`; a product then asks for its first weights while the kernel in front of it ends.  Weights that were
+    loaded once are at rest as soon as the host has waited for the device (`settle`)."""
+
+    __slots__ = ("data", "n", "k", "group", "zeros", "scale_dtype", "at_rest", "shape")
+    is_q4 = True
+
+    def __init__(self, data: torch.Tensor, n: int, k: int, group: int = 128, zeros: bool = False, scale_dtype: torch.dtype = torch.bfloat16,
+                 at_rest: bool = False):
+        want = (-(-n // ROWS), -(-k // K_BLOCK), block_bytes(group, scale_dtype, zeros))
+        if n < 1 or k < 1 or k % 8:
+            raise KernelError(f"4-bit weights [{n}, {k}]: the sizes are positive and the second a multiple of 8")
+        if data.dtype is not torch.uint8 or data.shape != want or not data.is_contiguous():
+            raise KernelError(f"4-bit weights [{n}, {k}] in groups of {group} are a contiguous uint8 {list(want)}, "
+                              f"not {data.dtype} {list(data.shape)}")
+        if data.data_ptr() % 16:
+            raise KernelError("4-bit weights start on a 16-byte boundary")
+        self.data, self.n, self.k, self.group, self.zeros, self.scale_dtype, self.at_rest = data, n, k, group, bool(zeros), scale_dtype, at_rest
+        self.shape = (n, k)
+
+    @property
+    def device(self):
+        return self.data.device
+
+    @property
+    def nbytes(self) -> int:
+        return self.data.numel()
+
+    def settle(self) -> "Q4Weight":
+        """Wait for the device; from here on the weights are at rest."""
+        if self.data.is_cuda:
+            torch.cuda.synchronize(self.data.device)
+        self.at_rest = True
+        return self
+
+    def _form(self):
+        return self.group, int(self.scale_dtype is torch.float32), int(self.zeros)
+
+
+def _device(t: torch.Tensor, *others: torch.Tensor) -> int:
+    if not t.is_cuda:
+        raise KernelError("kernel called with a CPU tensor: this engine has no CPU path")
+    index = t.get_device()
+    for o in others:
+        if not o.is_cuda or o.get_device() != index:
+            raise KernelError(f"tensors on different devices: {t.device} and {o.device}")
+    return index
+
+
+def _on(index: int):
+    """A context in which the device `index` is the current one, or None if it is already."""
+    return None if index == torch._C._cuda_getDevice() else torch.cuda.device(index)
+
+
+def quantize(w: torch.Tensor, group: int = 128, zeros: bool = False, scale_dtype: torch.dtype = torch.bfloat16) -> Q4Weight:
+    """A matrix [N, K], bfloat16 or float32, in 4 bits.  Of a group's values, with the scale rounded to its type (by way of float32):
+
+        without zeros   scale = max |w| / 7;  code = 8 + clamp(rint(w / scale), -7, 7)
+        with zeros      lo = min(0, min w), hi = max(0, max w), scale = (hi - lo) / 15;
+                        zero = clamp(rint(-lo / scale), 0, 15);  code = clamp(rint(w / scale) + zero, 0, 15)
+
+    rint takes ties to the even number.  A group of zeros stays zeros.  A group that holds an infinity or a value that is no number gets a
+    scale that is no number."""
+    if w.dim() != 2 or w.dtype not in (torch.bfloat16, torch.float32) or not w.is_contiguous():
+        raise KernelError(f"quantize takes a contiguous bfloat16 or float32 matrix, not {w.dtype} {list(w.shape)}")
+    index, (n, k) = _device(w), w.shape
+    size = block_bytes(group, scale_dtype, zeros)
+    if n < 1 or k < 1 or k % 8 or w.data_ptr() % 16:
+        raise KernelError(f"quantize: [{n}, {k}] needs positive sizes, the second a multiple of 8, and a base on a 16-byte boundary")
+    if (other := _on(index)) is not None:
+        with other:
+            return quantize(w, group, zeros, scale_dtype)
+    q = Q4Weight(torch.empty((-(-n // ROWS), -(-k // K_BLOCK), size), dtype=torch.uint8, device=w.device), n, k, group, zeros, scale_dtype)
+    _check(lib().tl_quantize_q4(w.data_ptr(), int(w.dtype is torch.float32), q.data.data_ptr(), n, k, *q._form(), _stream()), "quantize_q4")
+    return q
+
+
+def dequantize(w: Q4Weight, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    """The values that `w` stands for, [N, K]: float32, or those rounded to bfloat16."""
+    if dtype not in (torch.bfloat16, torch.float32):
+        raise KernelError(f"dequantize gives bfloat16 or float32, not {dtype}")
+    if (other := _on(_device(w.data))) is not None:
+        with other:
+            return dequantize(w, dtype)
+    out = torch.empty(w.shape, dtype=dtype, device=w.data.device)
+    _check(lib().tl_dequantize_q4(w.data.data_ptr(), out.data_ptr(), int(dtype is torch.float32), w.n, w.k, *w._form(), _stream()), "dequantize_q4")
+    return out
+
+
+def pack(codes: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor | None = None, group: int = 128) -> Q4Weight:
+    """Weights that were quantized elsewhere: codes [N, K] whole numbers 0..15, scales [N, ceil(K / group)] bfloat16 or float32, zeros (the
+    same shape) whole numbers 0..15 or None: 8.  Works where the tensors are, on the host too; values outside 0..15 are refused."""
+    if codes.dim() != 2 or codes.dtype.is_floating_point or codes.dtype.is_complex or codes.dtype == torch.bool:
+        raise KernelError(f"pack: codes are whole numbers [N, K], not {codes.dtype} {list(codes.shape)}")
+    n, k = codes.shape
+    size = block_bytes(group, scales.dtype, zeros is not None)
+    if n < 1 or k < 1 or k % 8:
+        raise KernelError(f"pack: [{n}, {k}] needs positive sizes, the second a multiple of 8")
+    per_row = (n, -(-k // group))
+    if tuple(scales.shape) != per_row or (zeros is not None and (tuple(zeros.shape) != per_row or zeros.dtype.is_floating_point)):
+        raise KernelError(f"pack: [{n}, {k}] in groups of {group} has scales (and whole zeros) of {list(per_row)}")
+    for what, t in (("codes", codes), ("zeros", zeros)):
+        if t is not None and (t.device != codes.device or bool(((t < 0) | (t > 15)).any())):
+            raise KernelError(f"pack: {what} are 0..15, on the codes' device")
+    if scales.device != codes.device:
+        raise KernelError("pack: scales are on the codes' device")
+    tiles, blocks, groups = -(-n // ROWS), -(-k // K_BLOCK), K_BLOCK // group
+    c = torch.full((tiles * ROWS, blocks * K_BLOCK), 8, dtype=torch.uint8, device=codes.device)
+    c[:n, :k] = codes.to(torch.uint8)
+    c = c.view(tiles, ROWS, blocks, 4, 4, 2, 2, 2).permute(0, 2, 3, 1, 4, 7, 5, 6)      # [tile, block, k / 32, row, word, h, p, q]
+    pieces = [(c[..., 0] | (c[..., 1] << 4)).reshape(tiles, blocks, CODE_BYTES)]
+
+    def by_block(t, fill):
+        full = torch.full((tiles * ROWS, blocks * groups), fill, dtype=t.dtype, device=t.device)
+        full[:n, :per_row[1]] = t
+        return full.view(tiles, ROWS, blocks, groups).permute(0, 2, 3, 1).contiguous().view(tiles, blocks, groups * ROWS)
+
+    pieces.append(by_block(scales, 0).view(torch.uint8))
+    if zeros is not None:
+        pieces.append(by_block(zeros.to(torch.uint8), 8))
+    data = torch.cat(pieces, dim=2)
+    assert data.shape[2] == size
+    return Q4Weight(data, n, k, group, zeros is not None, scales.dtype)
+
+
+_GATES = {"silu": 1, "gelu_tanh": 2, True: 1}
+
+
+def _gate(gated):
+    """`gated` False, True ("silu"), "gelu_tanh" or ("swish_clamped", limit, alpha): (code, limit, alpha)."""
+    if not gated:
+        return 0, 0.0, 1.0
+    if isinstance(gated, tuple):
+        if len(gated) == 3 and gated[0] == "swish_clamped" and gated[1] > 0:
+            return 3, float(gated[1]), float(gated[2])
+    elif gated in _GATES:
+        return _GATES[gated], 0.0, 1.0
+    raise KernelError(f"a gated epilogue applies 'silu', 'gelu_tanh' or ('swish_clamped', limit, alpha), not {gated!r}")
+
+
+def gemm_q4(x: torch.Tensor, w: Q4Weight, out_dtype: torch.dtype = torch.bfloat16, *, gated=False, out: torch.Tensor | None = None) -> torch.Tensor:
+    """x [T, K] bfloat16 times the matrix that `w` stands for, transposed: [T, N], bfloat16 or float32, sums in float32 and rounded once.
+    Rows of x may lie apart (a multiple of 8 values); T may be 0.
+    `gated` ("silu", "gelu_tanh" or ("swish_clamped", limit, alpha)): w holds gate and up rows alternating in blocks of 64 (N a multiple of
+    128), the result is act(gate) * up, [T, N / 2], from the float32 sums.  `out`: a tensor to write, of the result's shape and type, with rows
+    that may lie apart."""
+    gate, limit, alpha = _gate(gated)
+    if x.dtype is not torch.bfloat16 or x.dim() != 2 or x.shape[1] != w.k:
+        raise KernelError(f"gemm_q4: x is bfloat16 [T, {w.k}], not {x.dtype} {list(x.shape)}")
+    if out_dtype is not torch.bfloat16 and out_dtype is not torch.float32:
+        raise KernelError("gemm_q4: output is bfloat16 or float32")
+    if gate and w.n % 128:
+        raise KernelError(f"gemm_q4: gate and up rows alternate in blocks of 64, {w.n} rows are no multiple of 128")
+    index, T, n = _device(x, w.data), x.shape[0], w.n // 2 if gate else w.n
+    ldx = x.stride(0) if T > 1 else w.k
+    if T and ((x.stride(1) != 1 and w.k > 1) or ldx < w.k or ldx % 8 or x.data_ptr() % 16):
+        raise KernelError("gemm_q4: x has unit inner stride and rows that start on 16-byte boundaries, one behind the other")
+    if out is None:
+        out = torch.empty((T, n), dtype=out_dtype, device=x.device)
+        ldo = n
+    else:
+        ldo = out.stride(0) if T > 1 else n
+        if out.shape != (T, n) or out.dtype is not out_dtype or (n > 1 and out.stride(1) != 1) or (T > 1 and ldo < n):
+            raise KernelError(f"gemm_q4: out is {out_dtype} [{T}, {n}] with unit inner stride")
+        _device(x, out)
+    if T == 0:
+        return out
+    if (other := _on(index)) is not None:
+        with other:
+            return gemm_q4(x, w, out_dtype, gated=gated, out=out)
+    _check(lib().tl_gemm_q4(x.data_ptr(), ldx, w.data.data_ptr(), out.data_ptr(), out_dtype is torch.float32, ldo, T, w.n, w.k, w.group,
+                            w.scale_dtype is torch.float32, w.zeros, gate, limit, alpha, w.at_rest, device_status(x.device).data_ptr(), _stream()),
+           "gemm_q4+gated" if gate else "gemm_q4")
+    return out
+
+
+__all__ = ["Q4Weight", "block_bytes", "dequantize", "gemm_q4", "pack", "quantize", "lib"]

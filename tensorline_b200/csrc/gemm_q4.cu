@@ -225,17 +225,21 @@ gemm_q4_kernel(const __grid_constant__ CUtensorMap map_x, const Q4Args G) {
                 if (g == gs - 1 && lane == 0) { mbar_arrive(a_empty + i % NA); mbar_arrive(empty + s); }
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const uint32_t at = lanes + Sh::D_COL + c * BN;
+                constexpr int AT_ONCE = 16;
 #pragma unroll
-                for (int c0 = 0; c0 < BN; c0 += 16) {
-                    float r[16];
-                    q4_ld16(at + c0, r);
+                for (int c0 = 0; c0 < BN; c0 += AT_ONCE) {
+                    float r[AT_ONCE / 16][16];
+#pragma unroll
+                    for (int j = 0; j < AT_ONCE / 16; ++j) q4_ld16(at + c0 + 16 * j, r[j]);
                     tmem_ld_wait();
+                    if (c0 + AT_ONCE >= BN) {            // the last of them are in registers
+                        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(d_empty + c);
+                    }
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) acc[c0 + j] = fmaf(sc[g], r[j], acc[c0 + j]);
+                    for (int j = 0; j < AT_ONCE; j += 2) q4_fma2(sc[g], r[j / 16][j % 16], r[j / 16][j % 16 + 1], acc[c0 + j], acc[c0 + j + 1]);
                 }
-                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-                __syncwarp();
-                if (lane == 0) mbar_arrive(d_empty + c);
             }
             if (++s == S) { s = 0; ++turn; }
         }
@@ -337,16 +341,19 @@ TL_EXPORT int tl_q4_block_bytes(int group, int scale_f32, int zeros) {
     return q4_form(&f, group, scale_f32, zeros) ? f.bytes : 0;
 }
 
-// y[T, ldo] = x[T, ldx] w^T over weights of 4 bits, N x K.  `gate` 1..3: rows of w are gates and what they weigh, alternating in blocks of 64
-// (N % 128 == 0), and y [T, N / 2] is act(gate) * up: 1 silu, 2 the tanh form of gelu, 3 the clamped swish with `limit` and `alpha`.
-// `at_rest`: no kernel of this stream that could still be running writes the weights.  Returns 0, a CUDA error or 1 for what it does not take.
-TL_EXPORT int tl_gemm_q4(const void* x, long long ldx, const void* w, void* y, int out_f32, int ldo, int T, int N, int K, int group, int scale_f32,
-                         int zeros, int gate, float limit, float alpha, int at_rest, int* status, cudaStream_t stream) {
+// y[T, ldo] = x[T, ldx] w^T over weights of 4 bits, N x K.  `form`: k a group, and from bit 8 on: scales are float, there are zeros, (two bits) the
+// gate, y is float, no kernel of this stream that could still be running writes the weights.  Gate 1..3: rows of w are gates and what they
+// weigh, alternating in blocks of 64 (N % 128 == 0), and y [T, N / 2] is act(gate) * up: 1 silu, 2 the tanh form of gelu, 3 the clamped
+// swish with `limit` and `alpha`.  Returns 0, a CUDA error or 1 for what it does not take.
+TL_EXPORT int tl_gemm_q4(const void* x, long long ldx, const void* w, void* y, int ldo, int T, int N, int K, int form, float limit, float alpha,
+                         int* status, cudaStream_t stream) {
     Q4Args G{};
-    if (T < 0 || N < 1 || K < 1 || (K & 7) || !q4_form(&G.form, group, scale_f32, zeros)) return 1;
-    if (gate < 0 || gate > 3 || (gate && (N & 127)) || ldo < (gate ? N / 2 : N)) return 1;
+    const int gate = form >> 10 & 3, out_f32 = form >> 12 & 1;
+    if (form < 0 || form >> 14 || T < 0 || N < 1 || K < 1 || (K & 7) || !q4_form(&G.form, form & 255, form >> 8 & 1, form >> 9 & 1)) return 1;
+    if ((gate && (N & 127)) || ldo < (gate ? N / 2 : N)) return 1;
     if (T == 0) return 0;
     if (ldx < K || (ldx & 7) || ((uintptr_t)x & 15) || ((uintptr_t)w & 15) || !y || !status) return 1;
+    const int at_rest = form >> 13 & 1;
     int e = load_encode();
     if (e) return e;
     G.x = (const unsigned char*)x; G.ldx = ldx; G.w = (const unsigned char*)w; G.blocks = (K + Q4_K - 1) / Q4_K;

@@ -17,7 +17,7 @@ constexpr int QP_THREADS = 512;                          // warp 0: copies, 1: t
 constexpr int QP_REGS_COPY = 48, QP_REGS_UNPACK = 96, QP_REGS_SUM = 184;
 static_assert(QP_REGS_COPY + QP_REGS_UNPACK + 2 * QP_REGS_SUM <= 512, "a larger share would be waited for without end");
 constexpr int QP_MOST = 192, QP_CW = QP_MOST / 2;        // tokens of a pair, of a summing warp
-constexpr int QP_NA = 2, QP_ND = 2, QP_D_COL = QP_NA * 64;
+constexpr int QP_NA = 4, QP_ND = 2, QP_D_COL = QP_NA * 32;      // halves of unpacked blocks (64 k, 32 columns), groups' sums
 constexpr int QP_STAGES_MAX = 12, QP_SMEM = 226 * 1024, QP_HAND = 2 * 2 * 16 * 64 * 4;      // gates and what they weigh change places: [2][half][16][64]
 static_assert(QP_D_COL + QP_ND * QP_MOST <= 512, "tensor memory");
 
@@ -44,7 +44,7 @@ gemm_q4_pair_kernel(const __grid_constant__ CUtensorMap map_x, const QpArgs A) {
     uint64_t* x_full = w_full + S;                       // the leader's: both blocks' tokens
     uint64_t* empty = x_full + S;                        // 4 unpacking warps, 8 summing warps
     uint64_t* a_full = empty + S;                        // [NA] the leader's: 4 unpacking warps of both blocks
-    uint64_t* a_empty = a_full + NA;                     // [NA] 8 summing warps: its products are done
+    uint64_t* a_empty = a_full + NA;                     // [NA] the products
     uint64_t* d_full = a_empty + NA;                     // [ND] the products
     uint64_t* d_empty = d_full + ND;                     // [ND] the leader's: 8 summing warps of both blocks
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(d_empty + ND);
@@ -57,7 +57,7 @@ gemm_q4_pair_kernel(const __grid_constant__ CUtensorMap map_x, const QpArgs A) {
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < S; ++s) { mbar_init(w_full + s, 1); mbar_init(x_full + s, 1); mbar_init(empty + s, 12); }
-        for (int b = 0; b < NA; ++b) { mbar_init(a_full + b, 8); mbar_init(a_empty + b, 8); }
+        for (int b = 0; b < NA; ++b) { mbar_init(a_full + b, 8); mbar_init(a_empty + b, 1); }
         for (int b = 0; b < ND; ++b) { mbar_init(d_full + b, 1); mbar_init(d_empty + b, 16); }
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -115,31 +115,40 @@ gemm_q4_pair_kernel(const __grid_constant__ CUtensorMap map_x, const QpArgs A) {
             const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)((2 * Q4_ROWS) >> 4) << 24);
             const uint32_t one = pair_elect();
             grid_dependency_wait();                      // the bounded waits start counting once the tokens can land
-            int d = 0, s = 0, turn = 0, it = 0;
-            bool ok = true;
+            int d = 0, s = 0, turn = 0, n = 0;           // groups, stage and its round, halves so far
+            bool ok = true, x_there = false, a_there = false, d_there = false;
             for (int item = pair; item < items && ok; item += pairs) {
-                for (int c = 0; c < n_k && ok; ++c, ++it) {
-                    const int b = it % NA, gs = GROUPS == 1 || c + 1 < n_k ? GROUPS : last;
-                    ok = mbar_wait(x_full + s, turn & 1, abort_flag, G.status, 82) && mbar_wait(a_full + b, (it / NA) & 1, abort_flag, G.status, 82);
+                for (int c = 0; c < n_k && ok; ++c) {
+                    const int gs = GROUPS == 1 || c + 1 < n_k ? GROUPS : last;
+                    ok = x_there || mbar_wait(x_full + s, turn & 1, abort_flag, G.status, 82);
                     const uint64_t x = desc_kmajor(smem_addr(ring + (size_t)s * G.stage_bytes));
-                    const uint32_t a = tmem + b * 64;
-#pragma unroll
-                    for (int g = 0; g < GROUPS; ++g) {
-                        if (g >= gs || !ok) break;
-                        const int e = d % ND;
-                        if (d >= ND) ok = mbar_wait(d_empty + e, (d / ND - 1) & 1, abort_flag, G.status, 83);
-                        if (!ok) break;
-                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-#pragma unroll
-                        for (int k = 0; k < GROUP / 16; ++k) {
-                            constexpr int STEP = 16;     // 16 k: 8 columns of weights, 32 bytes of tokens (2 of a descriptor's units of 16)
-                            const int at = g * (GROUP / STEP) + k;
-                            qp_mma(tmem + QP_D_COL + e * QP_MOST, a + at * 8, x + (at >> 2) * (x_half / 16) + (at & 3) * 2, idesc, k > 0, one);
-                        }
-                        pair_commit(d_full + e, one);
-                        ++d;
-                    }
                     if (++s == S) { s = 0; ++turn; }
+#pragma unroll
+                    for (int h = 0; h < 2; ++h, ++n) {
+                        const int b = n % NA;
+                        ok = ok && (a_there || mbar_wait(a_full + b, (n / NA) & 1, abort_flag, G.status, 82));
+                        if (!ok) break;
+                        // whether the next ones are there is asked now: an answer takes 80 cycles, and these products longer
+                        a_there = q4_peek(a_full + (n + 1) % NA, ((n + 1) / NA) & 1);
+                        if (h == 1) x_there = q4_peek(x_full + s, turn & 1);
+                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                        const uint32_t a = tmem + b * 32;
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {    // 16 k: 8 columns of weights, 32 bytes of tokens (2 of a descriptor's units of 16)
+                            constexpr int STEPS = GROUP / 16;
+                            const int at = h * 4 + k, g = at / STEPS, e = d % ND;
+                            if (g >= gs) continue;
+                            if (at % STEPS == 0) {
+                                if (d >= ND && !d_there) ok = mbar_wait(d_empty + e, (d / ND - 1) & 1, abort_flag, G.status, 83);
+                                if (!ok) break;
+                                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                                d_there = d + 1 >= ND && q4_peek(d_empty + (d + 1) % ND, ((d + 1) / ND - 1) & 1);
+                            }
+                            qp_mma(tmem + QP_D_COL + e * QP_MOST, a + k * 8, x + h * (x_half / 16) + k * 2, idesc, at % STEPS > 0, one);
+                            if (at % STEPS == STEPS - 1) { pair_commit(d_full + e, one); ++d; }
+                        }
+                        if (ok) pair_commit(a_empty + b, one);
+                    }
                 }
             }
       }
@@ -149,13 +158,13 @@ gemm_q4_pair_kernel(const __grid_constant__ CUtensorMap map_x, const QpArgs A) {
         const int row = quarter * 32 + lane, zeros_at = Q4_CODES + GROUPS * Q4_ROWS * (G.form.scale_f32 ? 4 : 2);
         const uint32_t magic = q4_magic();
         if (!G.at_rest) grid_dependency_wait();
-        int s = 0, turn = 0, it = 0;
-        bool ok = true;
+        int s = 0, turn = 0, n = 0;
+        bool ok = true, w_there = false, a_there = false;
         for (int item = pair; item < items && ok; item += pairs) {
-            for (int c = 0; c < n_k; ++c, ++it) {
-                const int b = it % NA;
-                if (!mbar_wait(w_full + s, turn & 1, abort_flag, G.status, 84)) { ok = false; break; }
+            for (int c = 0; c < n_k && ok; ++c) {
+                if (!w_there && !mbar_wait(w_full + s, turn & 1, abort_flag, G.status, 84)) { ok = false; break; }
                 const unsigned char* st = ring + (size_t)s * G.stage_bytes + x_bytes;
+                uint64_t* done = empty + s;
                 uint4 q[4];
                 uint32_t z[4];
 #pragma unroll
@@ -163,10 +172,14 @@ gemm_q4_pair_kernel(const __grid_constant__ CUtensorMap map_x, const QpArgs A) {
                     q[j] = *reinterpret_cast<const uint4*>(st + (j * Q4_ROWS + row) * 16);
                     z[j] = ZEROS ? st[zeros_at + (j * 32 / GROUP) * Q4_ROWS + row] : 8u;
                 }
-                if (it >= NA && !mbar_wait(a_empty + b, (it / NA - 1) & 1, abort_flag, G.status, 84)) { ok = false; break; }
-                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                if (++s == S) { s = 0; ++turn; }
 #pragma unroll
-                for (int half = 0; half < 2; ++half) {
+                for (int half = 0; half < 2; ++half, ++n) {
+                    const int b = n % NA;
+                    if (n >= NA && !a_there && !mbar_wait(a_empty + b, (n / NA - 1) & 1, abort_flag, G.status, 84)) { ok = false; break; }
+                    a_there = n + 1 >= NA && q4_peek(a_empty + (n + 1) % NA, ((n + 1) / NA - 1) & 1);
+                    if (half == 1) w_there = q4_peek(w_full + s, turn & 1);
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                     uint32_t v[32];
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
@@ -177,13 +190,15 @@ gemm_q4_pair_kernel(const __grid_constant__ CUtensorMap map_x, const QpArgs A) {
                         q4_values(p.z, magic, zz, v + 16 * j + 8);
                         q4_values(p.w, magic, zz, v + 16 * j + 12);
                     }
-                    q4_st32(lanes + b * 64 + half * 32, v);
+                    q4_st32(lanes + b * 32, v);
+                    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0) {
+                        pair_arrive(pair_peer(smem_addr(a_full + b), 0));
+                        if (half == 1) mbar_arrive(done);
+                    }
                 }
-                asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-                __syncwarp();
-                if (lane == 0) { pair_arrive(pair_peer(smem_addr(a_full + b), 0)); mbar_arrive(empty + s); }
-                if (++s == S) { s = 0; ++turn; }
             }
         }
     } else {
@@ -191,27 +206,32 @@ gemm_q4_pair_kernel(const __grid_constant__ CUtensorMap map_x, const QpArgs A) {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(QP_REGS_SUM));
         const int row = quarter * 32 + lane, half = (warp - 8) >> 2, cw = BN / 2;
         grid_dependency_wait();                          // the output may still be read by the kernel in front
-        int s = 0, turn = 0, it = 0, d = 0;
-        bool ok = true;
+        int s = 0, turn = 0, d = 0;
+        bool ok = true, w_there = false, d_there = false;
         for (int item = pair; item < items && ok; item += pairs) {
             float acc[QP_CW];
 #pragma unroll
             for (int c = 0; c < QP_CW; ++c) acc[c] = 0.f;
-            for (int c = 0; c < n_k && ok; ++c, ++it) {
-                if (!mbar_wait(w_full + s, turn & 1, abort_flag, G.status, 85)) { ok = false; break; }
+            for (int c = 0; c < n_k && ok; ++c) {
+                if (!w_there && !mbar_wait(w_full + s, turn & 1, abort_flag, G.status, 85)) { ok = false; break; }
                 const unsigned char* scales = ring + (size_t)s * G.stage_bytes + x_bytes + Q4_CODES;
+                uint64_t* done = empty + s;
                 const int gs = GROUPS == 1 || c + 1 < n_k ? GROUPS : last;
                 float sc[GROUPS];
 #pragma unroll
                 for (int g = 0; g < GROUPS; ++g) sc[g] = g < gs ? q4_scale(scales, g * Q4_ROWS + row, G.form.scale_f32) : 0.f;
+                if (++s == S) { s = 0; ++turn; }
                 __syncwarp();
 #pragma unroll
                 for (int g = 0; g < GROUPS; ++g) {
                     if (g >= gs) break;
                     const int e = d % ND;
-                    if (!mbar_wait(d_full + e, (d / ND) & 1, abort_flag, G.status, 85)) { ok = false; break; }
+                    if (!d_there && !mbar_wait(d_full + e, (d / ND) & 1, abort_flag, G.status, 85)) { ok = false; break; }
                     ++d;
-                    if (g == gs - 1 && lane == 0) { mbar_arrive(a_empty + it % NA); mbar_arrive(empty + s); }      // the block's products are done
+                    if (g == gs - 1) {
+                        if (lane == 0) mbar_arrive(done);      // the block's products are done
+                        w_there = q4_peek(w_full + s, turn & 1);
+                    }
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                     const uint32_t at = lanes + QP_D_COL + e * QP_MOST + half * cw;
 #pragma unroll
@@ -220,14 +240,16 @@ gemm_q4_pair_kernel(const __grid_constant__ CUtensorMap map_x, const QpArgs A) {
                         float r[16];
                         q4_ld16(at + c0, r);
                         tmem_ld_wait();
+                        if (c0 + 16 >= cw) {             // the last of them are in registers
+                            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                            __syncwarp();
+                            if (lane == 0) pair_arrive(pair_peer(smem_addr(d_empty + e), 0));
+                            d_there = q4_peek(d_full + d % ND, (d / ND) & 1);
+                        }
 #pragma unroll
-                        for (int j = 0; j < 16; ++j) acc[c0 + j] = fmaf(sc[g], r[j], acc[c0 + j]);
+                        for (int j = 0; j < 16; j += 2) q4_fma2(sc[g], r[j], r[j + 1], acc[c0 + j], acc[c0 + j + 1]);
                     }
-                    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-                    __syncwarp();
-                    if (lane == 0) pair_arrive(pair_peer(smem_addr(d_empty + e), 0));
                 }
-                if (++s == S) { s = 0; ++turn; }
             }
             if (!ok) break;
             const int tile = 2 * (item / A.t_tiles) + (int)rank, t0 = (item % A.t_tiles) * BN + half * cw;

@@ -68,6 +68,22 @@ __device__ __forceinline__ __nv_bfloat162 q4_zero(uint32_t z) {
     return *reinterpret_cast<const __nv_bfloat162*>(&v);
 }
 
+// a += s x, b += s y: the pairs of float multiply-adds of this architecture
+__device__ __forceinline__ void q4_fma2(float s, float x, float y, float& a, float& b) {
+    asm("{\n\t.reg .b64 m, v, c;\n\t"
+        "mov.b64 m, {%2, %2};\n\tmov.b64 v, {%3, %4};\n\tmov.b64 c, {%0, %1};\n\t"
+        "fma.rn.f32x2 c, m, v, c;\n\t"
+        "mov.b64 {%0, %1}, c;\n\t}" : "+f"(a), "+f"(b) : "f"(s), "f"(x), "f"(y));
+}
+// Whether a barrier's phase is over, without waiting.  Asking takes 80 cycles, ready or not, so it is asked well before the answer is needed.
+__device__ __forceinline__ bool q4_peek(uint64_t* bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile("{\n\t.reg .pred p;\n\t"
+                 "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+                 "selp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(ok) : "r"(smem_addr(bar)), "r"(parity) : "memory");
+    return ok != 0;
+}
 __device__ __forceinline__ void q4_bulk(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
                  ::"r"(dst), "l"(src), "r"(bytes), "r"(smem_addr(bar)) : "memory");

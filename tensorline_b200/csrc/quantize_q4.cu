@@ -134,20 +134,20 @@ int q4_grid(dim3* grid, int N, int K) {
 
 }  // namespace
 
-// Weights of 4 bits [ceil(N / 128)][ceil(K / 128)][block] from w [N, K], bfloat16 or float; K % 8 == 0.
-TL_EXPORT int tl_quantize_q4(const void* w, int w_f32, void* out, int N, int K, int group, int scale_f32, int zeros, cudaStream_t stream) {
+// Weights of 4 bits [ceil(N / 128)][ceil(K / 128)][block] from w [N, K], bfloat16 or float; K % 8 == 0.  `form_bits`: k a group, from bit 8 on: scales are float, there are zeros.
+TL_EXPORT int tl_quantize_q4(const void* w, int w_f32, void* out, int N, int K, int form_bits, cudaStream_t stream) {
     Q4Form form;
     dim3 grid;
-    if (N < 1 || K < 1 || (K & 7) || !q4_form(&form, group, scale_f32, zeros) || !q4_grid(&grid, N, K) || ((uintptr_t)w & 15) || ((uintptr_t)out & 15)) return 1;
+    if (N < 1 || K < 1 || (K & 7) || form_bits < 0 || form_bits >> 10 || !q4_form(&form, form_bits & 255, form_bits >> 8 & 1, form_bits >> 9 & 1) || !q4_grid(&grid, N, K) || ((uintptr_t)w & 15) || ((uintptr_t)out & 15)) return 1;
     return w_f32 ? launch_after_wait(quantize_q4_kernel<float>, grid, dim3(QQ_THREADS), 0, stream, (const float*)w, (unsigned char*)out, N, K, (int)grid.x, form)
                  : launch_after_wait(quantize_q4_kernel<bf16>, grid, dim3(QQ_THREADS), 0, stream, (const bf16*)w, (unsigned char*)out, N, K, (int)grid.x, form);
 }
 
 // The values that weights of 4 bits stand for, [N, K] bfloat16 or float.
-TL_EXPORT int tl_dequantize_q4(const void* w, void* out, int out_f32, int N, int K, int group, int scale_f32, int zeros, cudaStream_t stream) {
+TL_EXPORT int tl_dequantize_q4(const void* w, void* out, int out_f32, int N, int K, int form_bits, cudaStream_t stream) {
     Q4Form form;
     dim3 grid;
-    if (N < 1 || K < 1 || (K & 7) || !q4_form(&form, group, scale_f32, zeros) || !q4_grid(&grid, N, K) || ((uintptr_t)w & 15) || ((uintptr_t)out & 15)) return 1;
+    if (N < 1 || K < 1 || (K & 7) || form_bits < 0 || form_bits >> 10 || !q4_form(&form, form_bits & 255, form_bits >> 8 & 1, form_bits >> 9 & 1) || !q4_grid(&grid, N, K) || ((uintptr_t)w & 15) || ((uintptr_t)out & 15)) return 1;
     return out_f32 ? launch_after_wait(dequantize_q4_kernel<float>, grid, dim3(QQ_THREADS), 0, stream, (const unsigned char*)w, (float*)out, N, K, (int)grid.x, form)
                    : launch_after_wait(dequantize_q4_kernel<bf16>, grid, dim3(QQ_THREADS), 0, stream, (const unsigned char*)w, (bf16*)out, N, K, (int)grid.x, form);
 }

@@ -27,9 +27,9 @@ _P, _I, _F, _L = ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_longlon
 SOURCES = ["gemm_q4.cu", "gemm_q4_pair.cu", "gemv_q4.cu", "quantize_q4.cu"]
 _SIGNATURES = {
     "tl_q4_block_bytes": [_I, _I, _I],
-    "tl_gemm_q4": [_P, _L, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _I, _F, _F, _I, _P, _P],
-    "tl_quantize_q4": [_P, _I, _P, _I, _I, _I, _I, _I, _P],
-    "tl_dequantize_q4": [_P, _P, _I, _I, _I, _I, _I, _I, _P],
+    "tl_gemm_q4": [_P, _L, _P, _P, _I, _I, _I, _I, _I, _F, _F, _P, _P],
+    "tl_quantize_q4": [_P, _I, _P, _I, _I, _I, _P],
+    "tl_dequantize_q4": [_P, _P, _I, _I, _I, _I, _P],
 }
 GROUPS = (32, 64, 128)
 ROWS = K_BLOCK = 128                                      # of a stored block
@@ -69,7 +69,7 @@ class Q4Weight:
     when a product is launched writes `data`; a product then asks for its first weights while the kernel in front of it ends.  Weights that were
     loaded once are at rest as soon as the host has waited for the device (`settle`)."""
 
-    __slots__ = ("data", "n", "k", "group", "zeros", "scale_dtype", "at_rest", "shape")
+    __slots__ = ("data", "n", "k", "group", "zeros", "scale_dtype", "at_rest", "shape", "form")
     is_q4 = True
 
     def __init__(self, data: torch.Tensor, n: int, k: int, group: int = 128, zeros: bool = False, scale_dtype: torch.dtype = torch.bfloat16,
@@ -84,6 +84,7 @@ class Q4Weight:
             raise KernelError("4-bit weights start on a 16-byte boundary")
         self.data, self.n, self.k, self.group, self.zeros, self.scale_dtype, self.at_rest = data, n, k, group, bool(zeros), scale_dtype, at_rest
         self.shape = (n, k)
+        self.form = group | (256 if scale_dtype is torch.float32 else 0) | (512 if zeros else 0)      # as the C entries take it
 
     @property
     def device(self):
@@ -99,9 +100,6 @@ class Q4Weight:
             torch.cuda.synchronize(self.data.device)
         self.at_rest = True
         return self
-
-    def _form(self):
-        return self.group, int(self.scale_dtype is torch.float32), int(self.zeros)
 
 
 def _device(t: torch.Tensor, *others: torch.Tensor) -> int:
@@ -138,7 +136,7 @@ def quantize(w: torch.Tensor, group: int = 128, zeros: bool = False, scale_dtype
         with other:
             return quantize(w, group, zeros, scale_dtype)
     q = Q4Weight(torch.empty((-(-n // ROWS), -(-k // K_BLOCK), size), dtype=torch.uint8, device=w.device), n, k, group, zeros, scale_dtype)
-    _check(lib().tl_quantize_q4(w.data_ptr(), int(w.dtype is torch.float32), q.data.data_ptr(), n, k, *q._form(), _stream()), "quantize_q4")
+    _check(lib().tl_quantize_q4(w.data_ptr(), int(w.dtype is torch.float32), q.data.data_ptr(), n, k, q.form, _stream()), "quantize_q4")
     return q
 
 
@@ -150,7 +148,7 @@ def dequantize(w: Q4Weight, dtype: torch.dtype = torch.float32) -> torch.Tensor:
         with other:
             return dequantize(w, dtype)
     out = torch.empty(w.shape, dtype=dtype, device=w.data.device)
-    _check(lib().tl_dequantize_q4(w.data.data_ptr(), out.data_ptr(), int(dtype is torch.float32), w.n, w.k, *w._form(), _stream()), "dequantize_q4")
+    _check(lib().tl_dequantize_q4(w.data.data_ptr(), out.data_ptr(), int(dtype is torch.float32), w.n, w.k, w.form, _stream()), "dequantize_q4")
     return out
 
 
@@ -190,54 +188,75 @@ def pack(codes: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor | None =
     return Q4Weight(data, n, k, group, zeros is not None, scales.dtype)
 
 
-_GATES = {"silu": 1, "gelu_tanh": 2, True: 1}
+_GATES = {"silu": 1 << 10, "gelu_tanh": 2 << 10, True: 1 << 10}
+_OUT_F32, _AT_REST = 1 << 12, 1 << 13
+_status: dict = {}                                        # device index -> address of its status word
 
 
 def _gate(gated):
-    """`gated` False, True ("silu"), "gelu_tanh" or ("swish_clamped", limit, alpha): (code, limit, alpha)."""
-    if not gated:
-        return 0, 0.0, 1.0
+    """`gated` as the C entry takes it: (bits, limit, alpha)."""
     if isinstance(gated, tuple):
         if len(gated) == 3 and gated[0] == "swish_clamped" and gated[1] > 0:
-            return 3, float(gated[1]), float(gated[2])
+            return 3 << 10, float(gated[1]), float(gated[2])
     elif gated in _GATES:
         return _GATES[gated], 0.0, 1.0
     raise KernelError(f"a gated epilogue applies 'silu', 'gelu_tanh' or ('swish_clamped', limit, alpha), not {gated!r}")
 
 
+# A call takes the host 7 us and the smallest products 5 us, so what is asked of a tensor is asked once, and nothing is built that the call does
+# not need (10.5 us with properties of the device and an argument for each of the weights' properties).
 def gemm_q4(x: torch.Tensor, w: Q4Weight, out_dtype: torch.dtype = torch.bfloat16, *, gated=False, out: torch.Tensor | None = None) -> torch.Tensor:
     """x [T, K] bfloat16 times the matrix that `w` stands for, transposed: [T, N], bfloat16 or float32, sums in float32 and rounded once.
     Rows of x may lie apart (a multiple of 8 values); T may be 0.
     `gated` ("silu", "gelu_tanh" or ("swish_clamped", limit, alpha)): w holds gate and up rows alternating in blocks of 64 (N a multiple of
     128), the result is act(gate) * up, [T, N / 2], from the float32 sums.  `out`: a tensor to write, of the result's shape and type, with rows
     that may lie apart."""
-    gate, limit, alpha = _gate(gated)
-    if x.dtype is not torch.bfloat16 or x.dim() != 2 or x.shape[1] != w.k:
-        raise KernelError(f"gemm_q4: x is bfloat16 [T, {w.k}], not {x.dtype} {list(x.shape)}")
-    if out_dtype is not torch.bfloat16 and out_dtype is not torch.float32:
+    n, k, data = w.n, w.k, w.data
+    form, limit, alpha = w.form, 0.0, 1.0
+    if gated:
+        bits, limit, alpha = _gate(gated)
+        form |= bits
+        if n % 128:
+            raise KernelError(f"gemm_q4: gate and up rows alternate in blocks of 64, {n} rows are no multiple of 128")
+    cols = n // 2 if gated else n
+    shape = x.shape
+    if x.dtype is not torch.bfloat16 or len(shape) != 2 or shape[1] != k:
+        raise KernelError(f"gemm_q4: x is bfloat16 [T, {k}], not {x.dtype} {list(shape)}")
+    if out_dtype is torch.float32:
+        form |= _OUT_F32
+    elif out_dtype is not torch.bfloat16:
         raise KernelError("gemm_q4: output is bfloat16 or float32")
-    if gate and w.n % 128:
-        raise KernelError(f"gemm_q4: gate and up rows alternate in blocks of 64, {w.n} rows are no multiple of 128")
-    index, T, n = _device(x, w.data), x.shape[0], w.n // 2 if gate else w.n
-    ldx = x.stride(0) if T > 1 else w.k
-    if T and ((x.stride(1) != 1 and w.k > 1) or ldx < w.k or ldx % 8 or x.data_ptr() % 16):
-        raise KernelError("gemm_q4: x has unit inner stride and rows that start on 16-byte boundaries, one behind the other")
-    if out is None:
-        out = torch.empty((T, n), dtype=out_dtype, device=x.device)
-        ldo = n
+    if w.at_rest:
+        form |= _AT_REST
+    index, T = x.get_device(), shape[0]
+    if index < 0 or data.get_device() != index:
+        _device(x, data)                                 # says which
+    ptr = x.data_ptr()
+    if T > 1:
+        ldx, inner = x.stride()
     else:
-        ldo = out.stride(0) if T > 1 else n
-        if out.shape != (T, n) or out.dtype is not out_dtype or (n > 1 and out.stride(1) != 1) or (T > 1 and ldo < n):
-            raise KernelError(f"gemm_q4: out is {out_dtype} [{T}, {n}] with unit inner stride")
+        ldx, inner = k, x.stride(1)
+    if T and (inner != 1 or ldx < k or ldx % 8 or ptr % 16):
+        raise KernelError("gemm_q4: x has unit inner stride and rows that start on 16-byte boundaries, one behind the other")
+    ldo = cols
+    if out is None:
+        out = x.new_empty((T, cols), dtype=out_dtype)
+    else:
+        if T > 1:
+            ldo = out.stride(0)
+        if out.shape != (T, cols) or out.dtype is not out_dtype or (cols > 1 and out.stride(1) != 1) or ldo < cols:
+            raise KernelError(f"gemm_q4: out is {out_dtype} [{T}, {cols}] with unit inner stride")
         _device(x, out)
     if T == 0:
         return out
-    if (other := _on(index)) is not None:
-        with other:
+    if index != torch._C._cuda_getDevice():
+        with torch.cuda.device(index):
             return gemm_q4(x, w, out_dtype, gated=gated, out=out)
-    _check(lib().tl_gemm_q4(x.data_ptr(), ldx, w.data.data_ptr(), out.data_ptr(), out_dtype is torch.float32, ldo, T, w.n, w.k, w.group,
-                            w.scale_dtype is torch.float32, w.zeros, gate, limit, alpha, w.at_rest, device_status(x.device).data_ptr(), _stream()),
-           "gemm_q4+gated" if gate else "gemm_q4")
+    status = _status.get(index)
+    if status is None:
+        status = _status[index] = device_status(x.device).data_ptr()
+    _check((_lib or lib()).tl_gemm_q4(ptr, ldx, data.data_ptr(), out.data_ptr(), ldo, T, n, k, form, limit, alpha, status,
+                                      torch._C._cuda_getCurrentRawStream(index)), "gemm_q4+gated" if gated else "gemm_q4")
     return out
 
 

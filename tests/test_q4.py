@@ -88,11 +88,11 @@ def test_bytes_of_a_block_are_those_of_the_library():
 def test_c_entries_refuse_what_they_do_not_take():
     """No pointer is looked at before the sizes: these end on the host."""
     lib, p = ops_q4.lib(), 1 << 20
-    good = dict(x=p, ldx=64, w=p, y=p, f32=0, ldo=128, T=2, N=128, K=64, group=64, sf=0, z=0, gate=0, limit=0.0, alpha=1.0, rest=1, status=p, stream=None)
-    for bad in (dict(T=-1), dict(N=0), dict(K=0), dict(K=60), dict(group=16), dict(gate=4), dict(gate=1, N=192), dict(ldo=100), dict(ldx=56),
-                dict(ldx=68), dict(x=p + 2), dict(w=p + 8), dict(y=None), dict(status=None)):
+    good = dict(x=p, ldx=64, w=p, y=p, ldo=128, T=2, N=128, K=64, form=64, limit=0.0, alpha=1.0, status=p, stream=None)
+    for bad in (dict(T=-1), dict(N=0), dict(K=0), dict(K=60), dict(form=16), dict(form=64 | 1 << 14), dict(form=-1), dict(form=64 | 1 << 10, N=192),
+                dict(ldo=100), dict(ldx=56), dict(ldx=68), dict(x=p + 2), dict(w=p + 8), dict(y=None), dict(status=None)):
         assert lib.tl_gemm_q4(*{**good, **bad}.values()) == 1, bad
     assert lib.tl_gemm_q4(*{**good, "T": 0}.values()) == 0
-    for args in ((p, 0, p, 0, 64, 64, 0, 0), (p, 0, p, 4, 60, 64, 0, 0), (p, 0, p, 4, 64, 16, 0, 0), (p + 8, 0, p, 4, 64, 64, 0, 0), (p, 0, p + 8, 4, 64, 64, 0, 0)):
-        assert lib.tl_quantize_q4(*args, None) == 1
-        assert lib.tl_dequantize_q4(args[0], args[2], *args[1:2], *args[3:], None) == 1
+    for w, out, n, k, form in ((p, p, 0, 64, 64), (p, p, 4, 60, 64), (p, p, 4, 64, 16), (p + 8, p, 4, 64, 64), (p, p + 8, 4, 64, 64), (p, p, 4, 64, 64 | 1 << 10)):
+        assert lib.tl_quantize_q4(w, 0, out, n, k, form, None) == 1
+        assert lib.tl_dequantize_q4(w, out, 0, n, k, form, None) == 1

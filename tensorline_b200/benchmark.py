@@ -139,12 +139,20 @@ def random_weights(cfg, device, seed=0):
     return out
 
 
-def weight_bytes_read_per_step(cfg, layers):
+def weight_options(a) -> dict:
+    return dict(weight_bits=4, quantize_head=a.quantize_head) if a.weight_bits else {}
+
+
+def weight_bytes_read_per_step(cfg, layers, options=None):
     """Bytes of weights one decode step reads: every matrix of every layer once, the output head, the
-    norms; embedding rows are a few KB and left out."""
+    norms; embedding rows are a few KB and left out.  `options`: of `weight_options`."""
     H, I, d = cfg.hidden_size, cfg.intermediate_size, cfg.head_dim
     nq, nkv = cfg.num_attention_heads, cfg.num_key_value_heads
     per_layer = (nq + 2 * nkv) * d * (H + 1) + nq * d * H + 3 * H * I + 2 * H
+    if options:                                          # half a byte a weight and two a group of 128
+        packed = 0.5 + 2 / 128
+        matrices, head = layers * (per_layer - 2 * H - (nq + 2 * nkv) * d), cfg.vocab_size * H
+        return int(packed * matrices + 2 * layers * (2 * H + (nq + 2 * nkv) * d) + (packed if options["quantize_head"] else 2) * head + 2 * H)
     return 2 * (layers * per_layer + cfg.vocab_size * H + H)
 
 
@@ -433,7 +441,7 @@ def run_ours(a):
     mix = workload == "mix"
     eng = Engine(cfg, dtype="bfloat16", weights=weights, block_size=PAGE, max_num_seqs=max_seqs,
                  max_batched_tokens=MIX["chunk"] if mix else 2048, max_model_len=context,
-                 num_blocks=max_seqs * (context // PAGE), prefix_caching=False, cuda_graphs=True)
+                 num_blocks=max_seqs * (context // PAGE), prefix_caching=False, cuda_graphs=True, **weight_options(a))
     del weights
     V = cfg.vocab_size
     K, W = a.steps, a.warmup
@@ -441,6 +449,8 @@ def run_ours(a):
     batch = a.batch
     sizes = {"layers": L, "layers_full": layers_full, "hidden": cfg.hidden_size, "heads": cfg.num_attention_heads,
              "kv_heads": cfg.num_key_value_heads, "head_dim": cfg.head_dim, "intermediate": cfg.intermediate_size, "vocab": V}
+    if a.weight_bits:
+        sizes["weights"] = "4 bits, groups of 128" + (", output head too" if a.quantize_head else ", output head bf16")
     peak_tf = pk.get("bf16_tflops_sustained") or pk["bf16_tflops"]
     if mix:
         sampler = ClockSampler(0)
@@ -515,10 +525,10 @@ def run_ours(a):
     print(f"[bench] prefill {PREFILL_TOKENS}: {pre_ms:.2f} ms", file=sys.stderr, flush=True)
     flops = prefill_flops(cfg, L, PREFILL_TOKENS)
     kv_bytes = batch * (ctx0 + W + K // 2) * eng.runner.cache_bytes_per_token()
-    step_bytes = weight_bytes_read_per_step(cfg, L) + kv_bytes
+    step_bytes = weight_bytes_read_per_step(cfg, L, weight_options(a)) + kv_bytes
     achieved = step_bytes / (ms * 1e-3) / 1e9
     line = {
-        "metric": f"decode tok/s at batch {batch} ({model['name']} bf16, context {context})", "value": round(value, 1), "unit": "tok/s",
+        "metric": f"decode tok/s at batch {batch} ({model['name']} bf16{', weights of 4 bits' if a.weight_bits else ''}, context {context})", "value": round(value, 1), "unit": "tok/s",
         "n_gpus": 1, "steps": K, "warmup": W, "ms_per_step": round(ms, 4), "higher_is_better": True,
         "scaling": "weak", "vs_baseline": None, "dtype": "bf16", "data": "synthetic", "impl": "ours",
         "config": dict(sizes, model=f"{model['name']} layer sizes, random weights", global_batch=batch, seq_len=context,
@@ -752,6 +762,8 @@ def main(argv=None):
     ap.add_argument("--only", choices=["all", "decode", "prefill"], default="all",
                     help="decode / prefill: a short run of that phase alone (for profilers); prints its own line")
     ap.add_argument("--batch", type=int, default=8, help="decode batch of the main measurement")
+    ap.add_argument("--weight-bits", type=int, choices=[4], default=None, help="the layers' matrices in 4 bits (groups of 128 without zeros)")
+    ap.add_argument("--quantize-head", action="store_true", help="with --weight-bits: the output head too")
     ap.add_argument("--profile", action="store_true", help="add milliseconds per kernel class of one eager decode and one prompt step (mix: of one mixed step)")
     ap.add_argument("--timeline", action="store_true",
                     help="print the time line of one captured decode step from the kernels' own stamps (needs TENSORLINE_B200_TRACE=1)")

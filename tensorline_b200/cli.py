@@ -34,6 +34,10 @@ def _generate_parser() -> argparse.ArgumentParser:
     ap.add_argument("--block-size", type=int, default=16)
     ap.add_argument("--num-blocks", type=int, default=None, help="KV pages (default: fit 60%% of free memory)")
     ap.add_argument("--kv-cache-gb", type=float, default=None, help="KV cache size (default: 60%% of free memory)")
+    ap.add_argument("--weight-bits", type=int, choices=[4], default=None, help="quantize the layers' matrices to 4 bits as they are loaded")
+    ap.add_argument("--weight-group", type=int, choices=[32, 64, 128], default=128, help="values that share a scale (with --weight-bits)")
+    ap.add_argument("--weight-zeros", action="store_true", help="a zero point beside every scale (with --weight-bits)")
+    ap.add_argument("--quantize-head", action="store_true", help="the output head in 4 bits too (with --weight-bits)")
     ap.add_argument("--no-cuda-graphs", action="store_true", help="run decode steps eagerly")
     ap.add_argument("--no-overlap", action="store_true", help="read every decode step back before the next one is launched")
     ap.add_argument("--graph-warmup-tokens", type=int, default=512,
@@ -73,7 +77,8 @@ def cmd_generate(argv) -> int:
     eng = Engine(a.model, a.device, a.dtype, tokenizer=tok, block_size=a.block_size, num_blocks=a.num_blocks,
                  max_num_seqs=a.max_num_seqs, max_batched_tokens=a.max_batched_tokens, max_model_len=a.max_model_len,
                  cuda_graphs=not a.no_cuda_graphs, prefix_caching=not a.no_prefix_caching, kv_cache_gb=a.kv_cache_gb,
-                 graph_warmup_tokens=a.graph_warmup_tokens, overlap=not a.no_overlap, seed=a.seed)
+                 graph_warmup_tokens=a.graph_warmup_tokens, overlap=not a.no_overlap, seed=a.seed, weight_bits=a.weight_bits,
+                 weight_group=a.weight_group, weight_zeros=a.weight_zeros, quantize_head=a.quantize_head)
     prompts = list(a.prompt) + [[int(t) for t in s.split(",") if t.strip()] for s in a.prompt_ids]
     if not prompts:
         print("tensorline: give --prompt or --prompt-ids", file=sys.stderr)

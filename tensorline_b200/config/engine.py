@@ -21,6 +21,10 @@ class EngineConfig:
     graph_warmup_tokens: int = 512      # kept for the command line; graphs here do not depend on context length
     overlap: bool = True
     seed: int = 0
+    weight_bits: int | None = None      # 4: the layers' matrices as 4-bit codes with group scales, quantized as they are loaded; None: as stored
+    weight_group: int = 128             # values that share a scale: 32, 64 or 128
+    weight_zeros: bool = False          # a zero point per group beside its scale
+    quantize_head: bool = False         # the output head in 4 bits too (a tied one beside the embedding table, which stays as it is)
 
     def resolved_dtype(self, model_dtype: str | None = None) -> str:
         d = {"auto": None, "bf16": "bfloat16", "fp32": "float32", "float": "float32"}.get(self.dtype, self.dtype)
@@ -35,3 +39,9 @@ class EngineConfig:
             raise ValueError(f"block_size {self.block_size}: must divide 64")
         if self.max_num_seqs < 1 or self.max_batched_tokens < 1 or self.max_model_len < 2:
             raise ValueError("max_num_seqs, max_batched_tokens and max_model_len must be positive")
+        if self.weight_bits not in (None, 4):
+            raise ValueError(f"weight_bits {self.weight_bits!r}: 4, or None for weights as they are stored")
+        if self.weight_group not in (32, 64, 128):
+            raise ValueError(f"weight_group {self.weight_group}: must be 32, 64 or 128")
+        if self.weight_bits is None and (self.weight_zeros or self.quantize_head):
+            raise ValueError("weight_zeros and quantize_head come with weight_bits")

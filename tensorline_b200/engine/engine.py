@@ -68,7 +68,9 @@ class Engine:
         self.options.validate()
         self.device = pick_device(device)
         act = {"bfloat16": torch.bfloat16, "float32": torch.float32}[self.options.resolved_dtype()]
-        self.rt = Runtime(self.device, act, self.options.block_size)
+        self.rt = Runtime(self.device, act, self.options.block_size, weight_bits=self.options.weight_bits,
+                          weight_group=self.options.weight_group, weight_zeros=self.options.weight_zeros,
+                          quantize_head=self.options.quantize_head)
         if weights is None:
             self.model_dir = Path(model)
             self.model, self.config = load_model(self.model_dir, self.rt)
@@ -77,6 +79,8 @@ class Engine:
             self.config = model
             self.model = build_model(model, self.rt)
             self.model.bind(weights)
+        if self.options.weight_bits is not None:         # the matrices as they were stored: their memory is the cache's
+            torch.cuda.empty_cache()
         self.tokenizer = tokenizer
         if self.options.max_model_len > (self.model.spec.max_position_embeddings or self.options.max_model_len):
             self.options.max_model_len = self.model.spec.max_position_embeddings

@@ -109,6 +109,11 @@ class Model:
             block.bind(weights, layer.prefix)
         self.final_norm.bind(weights, self.spec.final_norm_prefix)
         self.head.bind(weights, self.spec.head_prefix, self.embedding)
+        if self.rt.quantized:                            # nothing writes these any more: from here on products ask for them ahead of time
+            self.rt.quantized[0].settle()
+            for q in self.rt.quantized:
+                q.at_rest = True
+            self.rt.quantized.clear()
 
     # ---- caches
     def cache_needs(self) -> dict:

@@ -137,7 +137,7 @@ class PagedAttention(Part):
         nq, nkv, dk, dv, d = self.nq, self.nkv, self.dk, self.dv, self.d
         n = {k: f"{prefix}.{v}" for k, v in self.names.items()}
         heads = (("q", nq, dk), ("k", nkv, dk), ("v", nkv, dv))
-        self.w_qkv = self._compute_copy(torch.cat([_pad_heads(weights[n[k]], h, size, d) for k, h, size in heads], dim=0))
+        self.w_qkv = self._matrix(torch.cat([_pad_heads(weights[n[k]], h, size, d) for k, h, size in heads], dim=0))
         if self.qkv_bias:
             self.b_qkv = torch.cat([_pad_heads(weights[n[k + "_bias"]], h, size, d) for k, h, size in heads], dim=0).contiguous()
             if self.b_qkv.dtype not in (torch.float32, torch.bfloat16):
@@ -145,7 +145,9 @@ class PagedAttention(Part):
         w_o = weights[n["o"]]                            # [H, nq * dv]: zero columns behind every head's values
         if dv != d:
             w_o = _pad_heads(w_o.t().contiguous(), nq, dv, d).t()
-        self.w_o = self._compute_copy(w_o)
+        # in 4 bits only where no engine pads the heads: columns between them would move the groups that share a scale
+        whole = dv >= dk and dv % (64 if self.has_mix else 16) == 0
+        self.w_o = self._matrix(w_o) if whole else self._compute_copy(w_o)
         if self.qk_norm_eps is not None and self.qk_norm_weight:
             pad = torch.ones(d - dk, dtype=torch.float32, device=self.w_o.device)        # behind the head's own size: zeros stay zeros
             self.q_norm = torch.cat([weights[n["q_norm"]].float(), pad]).contiguous()

@@ -55,6 +55,11 @@ class Runtime:
     device: torch.device
     act_dtype: torch.dtype              # torch.float32 (true 32-bit engine) or torch.bfloat16
     page_size: int = 16
+    weight_bits: int | None = None      # 4: matrices that products read are quantized as they are bound
+    weight_group: int = 128
+    weight_zeros: bool = False
+    quantize_head: bool = False
+    quantized: list = field(default_factory=list)       # of the model that is being bound: at rest once the host has waited for them
 
     @property
     def exact(self) -> bool:
@@ -85,6 +90,19 @@ class Part:
         if self.rt.exact or t.dtype == torch.bfloat16:
             return t.contiguous()
         return t.to(torch.bfloat16).contiguous()
+
+    def _matrix(self, t: torch.Tensor):
+        """A matrix that only `matmul` reads: as `_compute_copy`, or in 4 bits (a `Q4Weight`) where the runtime says so.  The 32-bit engine
+        then reads the values that the 4-bit weights stand for, exactly.  Rows whose length is no multiple of 8 stay as they are."""
+        if self.rt.weight_bits != 4 or t.shape[1] % 8:
+            return self._compute_copy(t)
+        from .. import ops_q4
+        t = t.contiguous()
+        q = ops_q4.quantize(t.clone() if t.data_ptr() % 16 else t, self.rt.weight_group, self.rt.weight_zeros)
+        if self.rt.exact:
+            return ops_q4.dequantize(q)
+        self.rt.quantized.append(q)
+        return q
 
 
 class Registry:

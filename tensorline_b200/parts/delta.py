@@ -70,12 +70,12 @@ class GatedDelta(Part):
     def bind(self, weights, prefix):
         n = {k: f"{prefix}.{v}" for k, v in self.names.items()}
         # one stacked projection: q | k | v | gate | b | a; its float32 accumulators are what the recurrence reads
-        self.w_in = self._compute_copy(torch.cat([weights[n[k]] for k in ("q", "k", "v", "g", "b", "a")], dim=0))
+        self.w_in = self._matrix(torch.cat([weights[n[k]] for k in ("q", "k", "v", "g", "b", "a")], dim=0))
         self.taps_w = torch.cat([weights[n[k]] for k in ("q_conv", "k_conv", "v_conv")], dim=0).contiguous()
         self.A_log = weights[n["A_log"]].float().contiguous()
         self.dt_bias = weights[n["dt_bias"]].float().contiguous()
         self.head_weight = weights[n["norm"]].repeat(self.H).contiguous()      # one weight for all heads
-        self.w_o = self._compute_copy(weights[n["o"]])
+        self.w_o = self._matrix(weights[n["o"]])
         if self.rt.device.type == "cuda":
             if ops.delta_columns() != 16 or ops.delta_state_floats(self.d, self.compensated) != self._state_floats():
                 raise ops.KernelError("the delta kernel's state layout is not the one this mixer sizes its slots for")

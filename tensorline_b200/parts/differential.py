@@ -78,8 +78,8 @@ class DifferentialAttention(Part):
 
     def bind(self, weights, prefix):
         n = {k: f"{prefix}.{v}" for k, v in self.names.items()}
-        self.w_qkv = self._compute_copy(torch.cat([weights[n[k]] for k, _ in self._heads()], dim=0))
-        self.w_o = self._compute_copy(weights[n["o"]])
+        self.w_qkv = self._matrix(torch.cat([weights[n[k]] for k, _ in self._heads()], dim=0))
+        self.w_o = self._matrix(weights[n["o"]])
         if self.has_conv:
             self.taps_w = torch.cat([weights[n[k + "_conv"]] for k, _ in self._heads()], dim=0).contiguous()
         else:

@@ -94,9 +94,10 @@ class LMHead(Part):
 
     def bind(self, weights, prefix, embedding: Embedding | None = None):
         if self.tied:
-            self.weight = embedding.weight
+            self.weight = self._matrix(embedding.weight) if self.rt.quantize_head else embedding.weight
         else:
-            self.weight = self._compute_copy(weights[tensor_name(prefix, self.tensor)])
+            stored = weights[tensor_name(prefix, self.tensor)]
+            self.weight = self._matrix(stored) if self.rt.quantize_head else self._compute_copy(stored)
 
     def forward(self, h):
         logits = matmul(h, self.weight, out_dtype=torch.float32)

@@ -89,7 +89,7 @@ class LatentAttention(Part):
         if not self.reads_latent:
             down = ([weights[n["dq"]]] if self.qr else []) + [weights[n["dkv"]]] + \
                 ([weights[n["g"]]] if self.out_gate or self.head_gate else [])
-            self.w_down = self._compute_copy(torch.cat(down, dim=0))
+            self.w_down = self._matrix(torch.cat(down, dim=0))
             self.n_kv = weights[n["dkv_norm"]].contiguous()
         if self.has_sink:
             self.sink = weights[n["sink"]].float().contiguous()
@@ -97,10 +97,10 @@ class LatentAttention(Part):
         if self.head_gate and self.reads_latent:               # no down product: the gate's rows ride in the queries', padded to whole 16 bytes
             g = weights[n["g"]].to(uq.dtype)
             uq = torch.cat([uq, g, torch.zeros((-(uq.shape[0] + g.shape[0]) % 8, g.shape[1]), dtype=uq.dtype, device=uq.device)])
-        self.w_uq = self._compute_copy(uq)
+        self.w_uq = self._matrix(uq)
         self.w_uk = self._compute_copy(weights[n["uk"]].view(H, self.dk, self.rank))                       # [H, K = dk, N = rank]
         self.w_uv = self._compute_copy(weights[n["uv"]].view(H, self.dv, self.rank).transpose(1, 2))       # [H, K = rank, N = dv]
-        self.w_o = self._compute_copy(weights[n["o"]])
+        self.w_o = self._matrix(weights[n["o"]])
         self.n_q = weights[n["dq_norm"]].to(self.n_kv.dtype).contiguous() if self.qr else None
 
     def forward(self, h, ctx, cache):

@@ -1,5 +1,7 @@
 """Matrix products of the parts: y = x W^T, weights [out, in] (tensorline/quant.py:3).
 
+Weights of 4 bits (`Q4Weight`, bfloat16 engine) have products of their own at every number of tokens (`ops_q4.gemm_q4`).  For the others:
+
 The 32-bit engine uses the float products of this package (`ops.gemm_f32`), whose order of additions is fixed.  The bfloat16 engine has two
 routes, both with float32 accumulation:
   * the hand-written tcgen05 / TMA kernel (`csrc/gemm_tc.cu`) for steps of few tokens against large
@@ -14,7 +16,7 @@ import os
 
 import torch
 
-from .. import ops
+from .. import ops, ops_q4
 
 TC_MAX_TOKENS = int(os.environ.get("TENSORLINE_B200_TC_MAX_TOKENS", 64))     # the hand-written kernel wins up to this many tokens ...
 TC_MIN_WEIGHT_ELEMENTS = int(os.environ.get("TENSORLINE_B200_TC_MIN_ELEMENTS", 8 << 20))   # ... against matrices of at least this many elements
@@ -255,7 +257,11 @@ def resolve(t):
 def matmul(x, w: torch.Tensor, out_dtype: torch.dtype | None = None, may_defer: bool = False, to_residual: bool = False):
     """x [T, K] (float32 or bfloat16) times w [N, K]^T -> [T, N].  `may_defer`: the caller hands the
     result to a consumer that takes a `SplitSum`.  `to_residual`: the result is an addend of the residual stream and
-    goes to a norm's `add_norm`: a `PendingProduct` may come back instead of a result.  `x` may be a `NormedInput`."""
+    goes to a norm's `add_norm`: a `PendingProduct` may come back instead of a result.  `x` may be a `NormedInput`, `w` a `Q4Weight`."""
+    if isinstance(w, ops_q4.Q4Weight):                   # sums are whole and scaled in the product's own kernel: nothing is deferred
+        x = resolve(x)
+        plain = x.stride(1) == 1 and x.stride(0) % 8 == 0 and x.data_ptr() % 16 == 0
+        return ops_q4.gemm_q4(x if plain else x.clone(memory_format=torch.contiguous_format), w, out_dtype or x.dtype)
     if isinstance(x, NormedInput):
         if x.rows is None and use_tc(x.shape[0], w.shape[0], w.shape[1]) and w.dtype == torch.bfloat16:
             from .. import ops_gemm

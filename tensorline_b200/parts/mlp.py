@@ -13,7 +13,7 @@ from __future__ import annotations
 
 import torch
 
-from .. import ops
+from .. import ops, ops_q4
 from .base import Part, Runtime, TensorSpec, register_feed_forward
 from .linear import NormedInput, matmul, resolve, use_pair_product, use_tc
 
@@ -52,13 +52,15 @@ class GatedMLP(Part):
         self.block = GATE_BLOCK if (self.rt.act_dtype == torch.bfloat16 and I % GATE_BLOCK == 0) else None
         if self.block:
             gu = torch.stack((g.view(I // GATE_BLOCK, GATE_BLOCK, H), u.view(I // GATE_BLOCK, GATE_BLOCK, H)), dim=1)
-            self.w_gate_up = self._compute_copy(gu.reshape(2 * I, H))
+            self.w_gate_up = self._matrix(gu.reshape(2 * I, H))
         else:
-            self.w_gate_up = self._compute_copy(torch.cat((g, u), dim=0))
-        self.w_down = self._compute_copy(weights[f"{prefix}.{self.names['down']}"])
+            self.w_gate_up = self._matrix(torch.cat((g, u), dim=0))
+        self.w_down = self._matrix(weights[f"{prefix}.{self.names['down']}"])
 
     def forward(self, h, ctx):
         I = self.intermediate
+        if self.block and isinstance(self.w_gate_up, ops_q4.Q4Weight):         # 4 bits: both projections, the activation and the product in one kernel
+            return matmul(ops_q4.gemm_q4(resolve(h), self.w_gate_up, gated=self.gate), self.w_down)
         if isinstance(h, NormedInput) and h.rows is not None:
             h = h.materialize()
         if self.block and h.dtype == torch.bfloat16 and h.is_contiguous() and use_tc(h.shape[0], 2 * I, self.hidden):
@@ -99,8 +101,8 @@ class PlainMLP(Part):
         return {f"{prefix}.{n['up']}": TensorSpec((I, H)), f"{prefix}.{n['down']}": TensorSpec((H, I))}
 
     def bind(self, weights, prefix):
-        self.w_up = self._compute_copy(weights[f"{prefix}.{self.names['up']}"])
-        self.w_down = self._compute_copy(weights[f"{prefix}.{self.names['down']}"])
+        self.w_up = self._matrix(weights[f"{prefix}.{self.names['up']}"])
+        self.w_down = self._matrix(weights[f"{prefix}.{self.names['down']}"])
 
     def forward(self, h, ctx):
         m = self._inner(resolve(h))
@@ -108,7 +110,7 @@ class PlainMLP(Part):
 
     def _inner(self, h):
         T, I, H = h.shape[0], self.intermediate, self.hidden
-        if h.dtype == torch.bfloat16 and h.is_cuda and h.is_contiguous():
+        if h.dtype == torch.bfloat16 and h.is_cuda and h.is_contiguous() and not isinstance(self.w_up, ops_q4.Q4Weight):
             from .. import ops_gemm
             if use_tc(T, I, H) and ops_gemm.can_act(T, I, H):
                 return ops_gemm.gemm_tc(h, self.w_up, gated=self.act)

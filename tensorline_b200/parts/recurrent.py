@@ -78,8 +78,8 @@ class _MatrixState(Part):
 
     def bind(self, weights, prefix):
         n = self.names
-        self.w_in = self._compute_copy(torch.cat([weights[f"{prefix}.{n[k]}"] for k, _ in self._projections()], dim=0))
-        self.w_o = self._compute_copy(weights[f"{prefix}.{n['o']}"])
+        self.w_in = self._matrix(torch.cat([weights[f"{prefix}.{n[k]}"] for k, _ in self._projections()], dim=0))
+        self.w_o = self._matrix(weights[f"{prefix}.{n['o']}"])
         if self.rt.device.type == "cuda":
             if ops.scan_columns() != 16 or ops.scan_state_floats(self.d, self.gated) != self._state_floats():
                 raise ops.KernelError("the scan kernel's state layout is not the one this mixer sizes its slots for")

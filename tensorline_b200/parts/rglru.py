@@ -69,7 +69,7 @@ class RGLRU(Part):
     def bind(self, weights, prefix):
         n = {k: f"{prefix}.{v}" for k, v in self.names.items()}
         # one stacked projection: the gelu branch's rows, then the recurrent branch's
-        self.w_in = self._compute_copy(torch.cat([weights[n["y"]], weights[n["x"]]], dim=0))
+        self.w_in = self._matrix(torch.cat([weights[n["y"]], weights[n["x"]]], dim=0))
         self.b_in = torch.cat([weights[n["y_bias"]], weights[n["x_bias"]]]).float().contiguous()
         self.conv_w = weights[n["conv"]].float().contiguous()
         self.conv_b = weights[n["conv_bias"]].float().contiguous()
@@ -79,7 +79,7 @@ class RGLRU(Part):
         self.w_gates3 = self.w_gates.repeat(1, 3, 1).contiguous() if self.w_gates.dtype == torch.bfloat16 else None
         self.b_gates = torch.cat([weights[n["ra_bias"]], weights[n["ri_bias"]]], dim=1).float().contiguous()      # [blocks, 2 bw]
         self.lam = weights[n["lam"]].float().contiguous()
-        self.w_o = self._compute_copy(weights[n["o"]])
+        self.w_o = self._matrix(weights[n["o"]])
 
     def forward(self, h, ctx, cache):
         W, nb, bw = self.W, self.blocks, self.bw

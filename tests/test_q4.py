@@ -96,3 +96,16 @@ def test_c_entries_refuse_what_they_do_not_take():
     for w, out, n, k, form in ((p, p, 0, 64, 64), (p, p, 4, 60, 64), (p, p, 4, 64, 16), (p + 8, p, 4, 64, 64), (p, p + 8, 4, 64, 64), (p, p, 4, 64, 64 | 1 << 10)):
         assert lib.tl_quantize_q4(w, 0, out, n, k, form, None) == 1
         assert lib.tl_dequantize_q4(w, out, 0, n, k, form, None) == 1
+
+
+def test_options_of_the_command_and_the_engine():
+    from tensorline_b200 import cli
+    from tensorline_b200.config.engine import EngineConfig
+    a = cli._generate_parser().parse_args(["--model", "m", "--weight-bits", "4", "--weight-group", "64", "--weight-zeros", "--quantize-head"])
+    assert (a.weight_bits, a.weight_group, a.weight_zeros, a.quantize_head) == (4, 64, True, True)
+    a = cli._generate_parser().parse_args(["--model", "m"])
+    assert (a.weight_bits, a.weight_group, a.weight_zeros, a.quantize_head) == (None, 128, False, False)
+    EngineConfig(weight_bits=4, weight_group=32, weight_zeros=True, quantize_head=True).validate()
+    for bad in (dict(weight_bits=8), dict(weight_bits=4, weight_group=48), dict(weight_zeros=True), dict(quantize_head=True)):
+        with pytest.raises(ValueError):
+            EngineConfig(**bad).validate()

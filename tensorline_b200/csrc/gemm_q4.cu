@@ -14,7 +14,7 @@
 #include "q4.cuh"
 
 int gemv_q4(Q4Args G, cudaStream_t stream);                        // gemv_q4.cu
-int gemm_q4_pair(const Q4Args& G, int bn, cudaStream_t stream);     // gemm_q4_pair.cu
+int gemm_q4_long(const Q4Args& G, int bn, cudaStream_t stream);     // gemm_q4_long.cu
 
 namespace {
 
@@ -34,42 +34,24 @@ template <int BN> struct QgShape {
     static_assert(D_COL + ND * BN <= (int)COLS, "tensor memory");
 };
 
-__device__ __forceinline__ uint32_t qg_elect() {
-    uint32_t one;
-    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
-    return one;
-}
-// D (+)= A B with A in tensor memory; by a whole warp, the instruction itself by one lane (umma_pair.cuh has the reason)
-__device__ __forceinline__ void qg_mma(uint32_t acc, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate, uint32_t one) {
-    asm volatile("{\n\t.reg .pred p, q;\n\t"
-                 "setp.ne.b32 p, %4, 0;\n\t"
-                 "setp.ne.b32 q, %5, 0;\n\t"
-                 "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-                 ::"r"(acc), "r"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(one) : "memory");
-}
-__device__ __forceinline__ void qg_commit(uint64_t* bar, uint32_t one) {
-    asm volatile("{\n\t.reg .pred q;\n\t"
-                 "setp.ne.b32 q, %1, 0;\n\t"
-                 "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}"
-                 ::"r"(smem_addr(bar)), "r"(one) : "memory");
-}
 template <int BN, int GROUP, bool ZEROS>
 __global__ void __launch_bounds__(QgShape<BN>::THREADS, QgShape<BN>::PER_SM)
 gemm_q4_kernel(const __grid_constant__ CUtensorMap map_x, const Q4Args G) {
     using Sh = QgShape<BN>;
     constexpr int NA = Sh::NA, ND = Sh::ND, GROUPS = Q4_K / GROUP;
     extern __shared__ unsigned char smem_raw[];
-    unsigned char* ring = reinterpret_cast<unsigned char*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);      // a stage: tokens, then packed weights
+    __shared__ uint32_t tmem_slot;
+    __shared__ int abort_word;
+    volatile int* abort_flag = &abort_word;
+    const uint32_t ring = (smem_addr(smem_raw) + 1023) & ~1023u;             // a stage: tokens, then packed weights
     const int S = G.stages;
-    uint64_t* w_full = reinterpret_cast<uint64_t*>(ring + (size_t)S * G.stage_bytes);
-    uint64_t* x_full = w_full + S;
-    uint64_t* empty = x_full + S;                        // 4 unpacking warps, 4 summing warps
-    uint64_t* a_full = empty + S;                        // [NA] 4 unpacking warps
-    uint64_t* a_empty = a_full + NA;                     // [NA] 4 summing warps: its products are done
-    uint64_t* d_full = a_empty + NA;                     // [ND] the products
-    uint64_t* d_empty = d_full + ND;                     // [ND] 4 summing warps
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(d_empty + ND);
-    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    const uint32_t full = ring + S * G.stage_bytes;
+    const uint32_t empty = full + 8 * S;                 // 4 unpacking warps, 4 summing warps
+    const uint32_t a_full = empty + 8 * S;               // [NA] 4 unpacking warps
+    const uint32_t a_empty = a_full + 8 * NA;            // [NA] 4 summing warps: its products are done
+    const uint32_t d_full = a_empty + 8 * NA;            // [ND] the products
+    const uint32_t d_empty = d_full + 8 * ND;            // [ND] 4 summing warps
+    float* red = reinterpret_cast<float*>(smem_raw + (ring - smem_addr(smem_raw)));       // the sums, [token][row], in the ring once it is idle
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int tile = blockIdx.x, t0 = blockIdx.y * BN, nz = gridDim.z;
@@ -78,20 +60,20 @@ gemm_q4_kernel(const __grid_constant__ CUtensorMap map_x, const Q4Args G) {
     auto groups_of = [&](int i) { return GROUPS == 1 || i + 1 < n_k ? GROUPS : min(GROUPS, last); };
 
     if (threadIdx.x == 0) {
-        for (int s = 0; s < S; ++s) { mbar_init(w_full + s, 1); mbar_init(x_full + s, 1); mbar_init(empty + s, 8); }
-        for (int b = 0; b < NA; ++b) { mbar_init(a_full + b, 4); mbar_init(a_empty + b, 4); }
-        for (int b = 0; b < ND; ++b) { mbar_init(d_full + b, 1); mbar_init(d_empty + b, 4); }
-        *abort_flag = 0;
+        for (int s = 0; s < S; ++s) { q4_init(full + 8 * s, 1); q4_init(empty + 8 * s, 8); }
+        for (int b = 0; b < NA; ++b) { q4_init(a_full + 8 * b, 4); q4_init(a_empty + 8 * b, 4); }
+        for (int b = 0; b < ND; ++b) { q4_init(d_full + 8 * b, 1); q4_init(d_empty + 8 * b, 4); }
+        abort_word = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 1) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(tmem_slot)), "r"(Sh::COLS) : "memory");
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&tmem_slot)), "r"(Sh::COLS) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    const uint32_t tmem = *tmem_slot;
+    const uint32_t tmem = tmem_slot;
     const int quarter = warp & 3;                        // the lanes of tensor memory a warp reaches: 32 * (warp % 4)
     const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
     float acc[BN];                                       // of the summing warps: a row's outputs
@@ -102,14 +84,13 @@ gemm_q4_kernel(const __grid_constant__ CUtensorMap map_x, const Q4Args G) {
             asm volatile("prefetch.tensormap [%0];" ::"l"(&map_x) : "memory");
             const unsigned char* src = G.w + ((size_t)tile * G.blocks + k0) * G.form.bytes;
             auto load_w = [&](int i, int s) {
-                mbar_expect_tx(w_full + s, G.form.bytes);
-                q4_bulk(smem_addr(ring + (size_t)s * G.stage_bytes) + Sh::X_BYTES, src + (size_t)i * G.form.bytes, G.form.bytes, w_full + s);
+                q4_expect(full + 8 * s, Sh::X_BYTES + G.form.bytes);
+                q4_bulk(ring + s * G.stage_bytes + Sh::X_BYTES, src + (size_t)i * G.form.bytes, G.form.bytes, full + 8 * s);
             };
             auto load_x = [&](int i, int s) {
-                const uint32_t dst = smem_addr(ring + (size_t)s * G.stage_bytes);
-                mbar_expect_tx(x_full + s, Sh::X_BYTES);
-                tma_box(dst, &map_x, x_full + s, (k0 + i) * Q4_K, t0);
-                tma_box(dst + Sh::X_HALF, &map_x, x_full + s, (k0 + i) * Q4_K + 64, t0);
+                const uint32_t dst = ring + s * G.stage_bytes;
+                q4_box(dst, &map_x, full + 8 * s, (k0 + i) * Q4_K, t0);
+                q4_box(dst + Sh::X_HALF, &map_x, full + 8 * s, (k0 + i) * Q4_K + 64, t0);
             };
             const int ahead = min(n_k, S);
             if (!G.at_rest) grid_dependency_wait();
@@ -118,7 +99,7 @@ gemm_q4_kernel(const __grid_constant__ CUtensorMap map_x, const Q4Args G) {
             grid_dependency_trigger();
             for (int i = 0; i < ahead; ++i) load_x(i, i);
             for (int i = ahead, s = 0, turn = 0; i < n_k; ++i) {
-                if (!mbar_wait(empty + s, turn & 1, abort_flag, G.status, 71)) break;
+                if (!q4_wait(empty + 8 * s, turn & 1, abort_flag, G.status, 71)) break;
                 load_w(i, s);
                 load_x(i, s);
                 if (++s == S) { s = 0; ++turn; }
@@ -127,30 +108,30 @@ gemm_q4_kernel(const __grid_constant__ CUtensorMap map_x, const Q4Args G) {
     } else if (warp == 1) {
         // ---------------------------------------------------------------- products
         constexpr uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(Q4_ROWS >> 4) << 24);
-        const uint32_t one = qg_elect();
+        const uint32_t one = q4_elect();
         grid_dependency_wait();                          // the bounded waits start counting once the tokens can land
         int d = 0, s = 0, turn = 0;
         bool ok = true;
         for (int i = 0; i < n_k && ok; ++i) {
             const int b = i % NA;
-            ok = mbar_wait(x_full + s, turn & 1, abort_flag, G.status, 72) && mbar_wait(a_full + b, (i / NA) & 1, abort_flag, G.status, 72);
+            ok = q4_wait(a_full + 8 * b, (i / NA) & 1, abort_flag, G.status, 72);
             const int gs = groups_of(i);
-            const uint64_t x = desc_kmajor(smem_addr(ring + (size_t)s * G.stage_bytes));
+            const uint64_t x = desc_kmajor(ring + s * G.stage_bytes);
             const uint32_t a = tmem + b * 64;
 #pragma unroll
             for (int g = 0; g < GROUPS; ++g) {
                 if (g >= gs || !ok) break;
                 const int c = d % ND;
-                if (d >= ND) ok = mbar_wait(d_empty + c, (d / ND - 1) & 1, abort_flag, G.status, 73);
+                if (d >= ND) ok = q4_wait(d_empty + 8 * c, (d / ND - 1) & 1, abort_flag, G.status, 73);
                 if (!ok) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll
                 for (int k = 0; k < GROUP / 16; ++k) {
                     constexpr int STEP = 16;             // 16 k: 8 columns of weights, 32 bytes of tokens (2 of a descriptor's units of 16)
                     const int at = g * (GROUP / STEP) + k;
-                    qg_mma(tmem + Sh::D_COL + c * BN, a + at * 8, x + ((at >> 2) * Sh::X_HALF + (at & 3) * 32) / 16, idesc, k > 0, one);
+                    q4_mma(tmem + Sh::D_COL + c * BN, a + at * 8, x + ((at >> 2) * Sh::X_HALF + (at & 3) * 32) / 16, idesc, k > 0, one);
                 }
-                qg_commit(d_full + c, one);
+                q4_commit(d_full + 8 * c, one);
                 ++d;
             }
             if (!ok) break;
@@ -165,16 +146,16 @@ gemm_q4_kernel(const __grid_constant__ CUtensorMap map_x, const Q4Args G) {
         for (; i < n_k; i += Sh::UG) {
             const int b = i % NA;
             while (s >= S) { s -= S; ++turn; }
-            if (!mbar_wait(w_full + s, turn & 1, abort_flag, G.status, 74)) break;
-            const unsigned char* st = ring + (size_t)s * G.stage_bytes + Sh::X_BYTES;
+            if (!q4_wait(full + 8 * s, turn & 1, abort_flag, G.status, 74)) break;
+            const uint32_t st = ring + s * G.stage_bytes + Sh::X_BYTES;
             uint4 q[4];
             uint32_t z[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                q[j] = *reinterpret_cast<const uint4*>(st + (j * Q4_ROWS + row) * 16);
-                z[j] = ZEROS ? st[zeros_at + (j * 32 / GROUP) * Q4_ROWS + row] : 8u;
+                q[j] = q4_lds128(st + (j * Q4_ROWS + row) * 16);
+                z[j] = ZEROS ? q4_lds8(st + zeros_at + (j * 32 / GROUP) * Q4_ROWS + row) : 8u;
             }
-            if (i >= NA && !mbar_wait(a_empty + b, (i / NA - 1) & 1, abort_flag, G.status, 74)) break;
+            if (i >= NA && !q4_wait(a_empty + 8 * b, (i / NA - 1) & 1, abort_flag, G.status, 74)) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
@@ -191,13 +172,13 @@ gemm_q4_kernel(const __grid_constant__ CUtensorMap map_x, const Q4Args G) {
                 q4_st32(lanes + b * 64 + half * 32, v);
                 if (half == 0) {                         // the codes are in registers: the stage is free
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(empty + s);
+                    if (lane == 0) q4_arrive(empty + 8 * s);
                 }
             }
             asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             __syncwarp();
-            if (lane == 0) mbar_arrive(a_full + b);
+            if (lane == 0) q4_arrive(a_full + 8 * b);
             s += Sh::UG;
         }
     } else {
@@ -207,23 +188,20 @@ gemm_q4_kernel(const __grid_constant__ CUtensorMap map_x, const Q4Args G) {
         for (int c = 0; c < BN; ++c) acc[c] = 0.f;
         grid_dependency_wait();                          // the output may still be read by the kernel in front
         bool ok = true;
-        for (int i = 0, s = 0, turn = 0, d = 0; i < n_k && ok; ++i) {
-            if (!mbar_wait(w_full + s, turn & 1, abort_flag, G.status, 75)) { ok = false; break; }
-            const unsigned char* scales = ring + (size_t)s * G.stage_bytes + Sh::X_BYTES + Q4_CODES;
+        for (int i = 0, s = 0, d = 0; i < n_k && ok; ++i) {
+            const uint32_t scales = ring + s * G.stage_bytes + Sh::X_BYTES + Q4_CODES, done = empty + 8 * s;
             const int gs = groups_of(i);
-            float sc[GROUPS];
-#pragma unroll
-            for (int g = 0; g < GROUPS; ++g) sc[g] = g < gs ? q4_scale(scales, g * Q4_ROWS + row, G.form.scale_f32) : 0.f;
+            if (++s == S) s = 0;
 #pragma unroll
             for (int g = 0; g < GROUPS; ++g) {
                 if (g >= gs) break;
                 const int c = d % ND;
-                if (!mbar_wait(d_full + c, (d / ND) & 1, abort_flag, G.status, 75)) { ok = false; break; }
+                // over when the products are, and so is the stage's copy, which they came after
+                if (!q4_wait(d_full + 8 * c, (d / ND) & 1, abort_flag, G.status, 75)) { ok = false; break; }
                 ++d;
-                // The block's last products are done, and so are its unpacked weights and its stage.  (A commit a barrier, by the warp that issues
-                // the products, took that warp some 150 cycles each.)
-                if (g == gs - 1 && lane == 0) { mbar_arrive(a_empty + i % NA); mbar_arrive(empty + s); }
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                if (g == gs - 1 && lane == 0) q4_arrive(a_empty + 8 * (i % NA));
+                const float sc = q4_lds_scale(scales, g * Q4_ROWS + row, G.form.scale_f32);
                 const uint32_t at = lanes + Sh::D_COL + c * BN;
                 constexpr int AT_ONCE = 16;
 #pragma unroll
@@ -235,13 +213,15 @@ gemm_q4_kernel(const __grid_constant__ CUtensorMap map_x, const Q4Args G) {
                     if (c0 + AT_ONCE >= BN) {            // the last of them are in registers
                         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                         __syncwarp();
-                        if (lane == 0) mbar_arrive(d_empty + c);
+                        if (lane == 0) {
+                            q4_arrive(d_empty + 8 * c);
+                            if (g == gs - 1) q4_arrive(done);
+                        }
                     }
 #pragma unroll
-                    for (int j = 0; j < AT_ONCE; j += 2) q4_fma2(sc[g], r[j / 16][j % 16], r[j / 16][j % 16 + 1], acc[c0 + j], acc[c0 + j + 1]);
+                    for (int j = 0; j < AT_ONCE; j += 2) q4_fma2(sc, r[j / 16][j % 16], r[j / 16][j % 16 + 1], acc[c0 + j], acc[c0 + j + 1]);
                 }
             }
-            if (++s == S) { s = 0; ++turn; }
         }
         asm volatile("bar.sync 1, 128;" ::: "memory");   // the other summing warps have read their scales out of the ring
         if (ok && nz == 1 && !G.gate) {
@@ -252,14 +232,13 @@ gemm_q4_kernel(const __grid_constant__ CUtensorMap map_x, const Q4Args G) {
                     if (t0 + c < G.T) q4_store(G, (size_t)(t0 + c) * G.ldo + n, acc[c]);
             }
         } else if (ok) {                                 // the sums to shared memory, [token][row]: the ring is idle, every copy has been waited for
-            float* red = reinterpret_cast<float*>(ring);
 #pragma unroll
             for (int c = 0; c < BN; ++c) red[c * Q4_ROWS + row] = acc[c];
         }
     }
     if (nz > 1 || G.gate) {
         if (nz > 1) pair_cluster_sync(); else __syncthreads();
-        if (warp >= 2 && !*abort_flag) q4_finish<1, BN>(G, reinterpret_cast<const float*>(ring), tile, t0, nz, blockIdx.z, (int)threadIdx.x - 64, Sh::THREADS - 64);
+        if (warp >= 2 && !*abort_flag) q4_finish<1, BN>(G, red, tile, t0, nz, blockIdx.z, (int)threadIdx.x - 64, Sh::THREADS - 64);
         if (nz > 1) pair_cluster_sync();                 // nobody leaves while its shared memory is read
     }
     // -------------------------------------------------------------------- teardown
@@ -278,7 +257,7 @@ gemm_q4_kernel(const __grid_constant__ CUtensorMap map_x, const Q4Args G) {
 template <int BN, int GROUP, bool ZEROS>
 int qg_launch(const CUtensorMap& map, Q4Args G, int tiles, int splits, cudaStream_t stream) {
     using Sh = QgShape<BN>;
-    constexpr int BARS = (3 * QG_STAGES_MAX + 2 * Sh::NA + 2 * Sh::ND) * 8 + 16;
+    constexpr int BARS = (2 * QG_STAGES_MAX + 2 * Sh::NA + 2 * Sh::ND) * 8 + 16;
     static bool raised[TL_MAX_DEVICES] = {};
     int e = tl_raise_smem(gemm_q4_kernel<BN, GROUP, ZEROS>, raised, Sh::SMEM_MOST);
     if (e) return e;
@@ -319,16 +298,23 @@ int qg_launch_form(const CUtensorMap& map, const Q4Args& G, int tiles, int split
            G.form.group == 64 ? qg_launch<BN, 64, false>(map, G, tiles, splits, stream) : qg_launch<BN, 32, false>(map, G, tiles, splits, stream);
 }
 
-// Tokens of a tile on a pair of blocks: those that the pairs are done with first.  A tile's block of k takes 4 cycles a token, but no less
-// than about 700 (gemm_q4_pair.cu).
-int qg_pair_tokens(int T, int N) {
-    const int pairs = tl_num_sms() / 2, m_tiles = (N + 2 * Q4_ROWS - 1) / (2 * Q4_ROWS);
+// Tokens of a tile of gemm_q4_long.cu, 0: ranges of K in clusters (this file) are faster.  Its blocks, one a SM, take a block of k through in about
+// 370 + 1.1 ns a token (measured 410, 434, 480 and 510 ns at 32, 64, 96 and 128 tokens), so it is the tile with which they are done first.
+// With fewer tiles than half of the SMs, ranges of K in clusters may be done before it: a block of k 540 ns there and 13 us for the rest.  Measured,
+// us, here / there:  128 tokens, 28 tiles x 148 blocks of k 44 / 65;  74 x 28 22.5 / 17.9;  256 tokens, 28 x 148 50 / 68;  200 tokens, 36 x 28 21.3 / 17.5.
+int qg_tile_tokens(int T, int N, int blocks) {
+    const int sms = tl_num_sms(), m_tiles = (N + Q4_ROWS - 1) / Q4_ROWS;
     int best = 0;
-    long long least = 0;
-    for (int bn = 192; bn >= 32; bn -= 32) {
-        const long long items = (long long)m_tiles * ((T + bn - 1) / bn), rounds = (items + pairs - 1) / pairs;
-        const long long cost = rounds * (bn > 175 ? 4 * bn : 700);
+    long long least = 0;                                 // tenths of ns
+    for (int bn = 128; bn >= 32; bn -= 32) {
+        const long long items = (long long)m_tiles * ((T + bn - 1) / bn), rounds = (items + sms - 1) / sms;
+        const long long cost = rounds * blocks * (3700 + 11 * bn) + 40000;
         if (!best || cost < least) { best = bn; least = cost; }
+    }
+    const long long here = (long long)m_tiles * ((T + 127) / 128);
+    if (here * 2 <= sms) {
+        const long long ranges = sms / here < 8 ? sms / here : 8;
+        if ((blocks + ranges - 1) / ranges * 5400 + 130000 < least) return 0;
     }
     return best;
 }
@@ -360,7 +346,8 @@ TL_EXPORT int tl_gemm_q4(const void* x, long long ldx, const void* w, void* y, i
     G.out = y; G.out_f32 = out_f32; G.ldo = ldo; G.N = N; G.K = K; G.T = T;
     G.gate = gate; G.limit = limit; G.alpha = alpha; G.at_rest = at_rest; G.status = status;
     if (T <= Q4_FEW) return gemv_q4(G, stream);
-    if (T > Q4_SINGLE) return gemm_q4_pair(G, qg_pair_tokens(T, N), stream);
+    if (T > 64)
+        if (const int tokens = qg_tile_tokens(T, N, G.blocks)) return gemm_q4_long(G, tokens, stream);
     const int bn = T <= 16 ? 16 : T <= 32 ? 32 : T <= 64 ? 64 : 128;
     const int tiles = (N + Q4_ROWS - 1) / Q4_ROWS, t_tiles = (T + bn - 1) / bn;
     if (t_tiles > 65535) return 1;

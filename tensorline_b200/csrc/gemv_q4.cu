@@ -49,7 +49,7 @@ gemv_q4_kernel(const __grid_constant__ CUtensorMap map_x, const Q4Args G) {
             auto load_w = [&](int i, int s) {
                 const uint32_t bytes = min(GV_GROUPS, n_k - i * GV_GROUPS) * G.form.bytes;
                 mbar_expect_tx(full + s, X_BYTES + bytes);
-                q4_bulk(smem_addr(ring + (size_t)s * G.stage_bytes) + X_BYTES, src + (size_t)i * GV_GROUPS * G.form.bytes, bytes, full + s);
+                q4_bulk(smem_addr(ring + (size_t)s * G.stage_bytes) + X_BYTES, src + (size_t)i * GV_GROUPS * G.form.bytes, bytes, smem_addr(full + s));
             };
             auto load_x = [&](int i, int s) {
                 tma_box(smem_addr(ring + (size_t)s * G.stage_bytes), &map_x, full + s, (k0 + i * GV_GROUPS) * Q4_K, 0);

@@ -30,7 +30,6 @@ namespace {
 
 constexpr int Q4_ROWS = 128, Q4_K = 128, Q4_CODES = Q4_ROWS * Q4_K / 2;
 constexpr int Q4_FEW = 16;                                // tokens up to which gemv_q4.cu takes a product
-constexpr int Q4_SINGLE = 128;                            // tokens up to which one block a tile does (gemm_q4.cu)
 
 // 0 if there is no such form
 inline int q4_form(Q4Form* f, int group, int scale_f32, int zeros) {
@@ -68,6 +67,76 @@ __device__ __forceinline__ __nv_bfloat162 q4_zero(uint32_t z) {
     return *reinterpret_cast<const __nv_bfloat162*>(&v);
 }
 
+__device__ __forceinline__ uint32_t q4_elect() {
+    uint32_t one;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+    return one;
+}
+// D (+)= A B with A in tensor memory; by a whole warp, the instruction itself by one lane (umma_pair.cuh has the reason)
+__device__ __forceinline__ void q4_mma(uint32_t acc, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate, uint32_t one) {
+    asm volatile("{\n\t.reg .pred p, q;\n\t"
+                 "setp.ne.b32 p, %4, 0;\n\t"
+                 "setp.ne.b32 q, %5, 0;\n\t"
+                 "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+                 ::"r"(acc), "r"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(one) : "memory");
+}
+__device__ __forceinline__ void q4_commit(uint32_t bar, uint32_t one) {
+    asm volatile("{\n\t.reg .pred q;\n\t"
+                 "setp.ne.b32 q, %1, 0;\n\t"
+                 "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}"
+                 ::"r"(bar), "r"(one) : "memory");
+}
+
+// Shared memory by its 32-bit addresses.  (A pointer whose alignment was rounded up by hand is a generic one to the compiler: loads through it took
+// the long way, and every barrier's address was made again from 64 bits.)
+__device__ __forceinline__ uint4 q4_lds128(uint32_t at) {
+    uint4 v;
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at));
+    return v;
+}
+__device__ __forceinline__ uint32_t q4_lds8(uint32_t at) {
+    uint32_t v;
+    asm volatile("ld.shared.u8 %0, [%1];" : "=r"(v) : "r"(at));
+    return v;
+}
+__device__ __forceinline__ float q4_lds_scale(uint32_t scales, int at, int f32) {
+    if (f32) {
+        float v;
+        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(scales + 4 * at));
+        return v;
+    }
+    uint16_t v;
+    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(scales + 2 * at));
+    return __uint_as_float((uint32_t)v << 16);
+}
+__device__ __forceinline__ bool q4_try(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile("{\n\t.reg .pred p;\n\t"
+                 "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+                 "selp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    return ok != 0;
+}
+// as mbar_wait
+__device__ __forceinline__ bool q4_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* status, int code) {
+    if (q4_try(bar, parity)) return true;
+    const long long t0 = clock64();
+    while (!q4_try(bar, parity)) {
+        if (*abort_flag) return false;
+        if (clock64() - t0 > WAIT_CYCLES) {
+            *abort_flag = 1;
+            atomicCAS(status, 0, code);
+            return false;
+        }
+    }
+    return true;
+}
+__device__ __forceinline__ void q4_arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
+__device__ __forceinline__ void q4_expect(uint32_t bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void q4_init(uint32_t bar, uint32_t count) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count)); }
+
 // a += s x, b += s y: the pairs of float multiply-adds of this architecture
 __device__ __forceinline__ void q4_fma2(float s, float x, float y, float& a, float& b) {
     asm("{\n\t.reg .b64 m, v, c;\n\t"
@@ -75,18 +144,13 @@ __device__ __forceinline__ void q4_fma2(float s, float x, float y, float& a, flo
         "fma.rn.f32x2 c, m, v, c;\n\t"
         "mov.b64 {%0, %1}, c;\n\t}" : "+f"(a), "+f"(b) : "f"(s), "f"(x), "f"(y));
 }
-// Whether a barrier's phase is over, without waiting.  Asking takes 80 cycles, ready or not, so it is asked well before the answer is needed.
-__device__ __forceinline__ bool q4_peek(uint64_t* bar, uint32_t parity) {
-    uint32_t ok;
-    asm volatile("{\n\t.reg .pred p;\n\t"
-                 "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-                 "selp.u32 %0, 1, 0, p;\n\t}"
-                 : "=r"(ok) : "r"(smem_addr(bar)), "r"(parity) : "memory");
-    return ok != 0;
+__device__ __forceinline__ void q4_box(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y) {
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+                 ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y) : "memory");
 }
-__device__ __forceinline__ void q4_bulk(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
+__device__ __forceinline__ void q4_bulk(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-                 ::"r"(dst), "l"(src), "r"(bytes), "r"(smem_addr(bar)) : "memory");
+                 ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
 }
 __device__ __forceinline__ const float* q4_peer(const float* p, int rank) {      // the same shared-memory location in block `rank` of the cluster
     uint64_t out;

@@ -187,9 +187,9 @@ STATUS_ROLES = {1: "tcgen05 product: the copy thread waited for a free stage", 2
                 73: "4-bit product: the MMA warp waited for a free accumulator", 74: "4-bit product: the unpacking waited for weights or for room",
                 75: "4-bit product: the sums waited for weights or an accumulator",
                 76: "4-bit product of few tokens: the copy thread waited for a free stage", 77: "4-bit product of few tokens: a warp waited for a stage's copies",
-                81: "two-block 4-bit product: a copy thread waited for a free stage", 82: "two-block 4-bit product: the MMA warp waited for tokens or weights",
-                83: "two-block 4-bit product: the MMA warp waited for a free accumulator", 84: "two-block 4-bit product: the unpacking waited for weights or for room",
-                85: "two-block 4-bit product: the sums waited for weights or an accumulator",
+                81: "4-bit product of many tokens: a copy thread waited for a free stage", 82: "4-bit product of many tokens: the MMA warp waited for tokens or weights",
+                83: "4-bit product of many tokens: the MMA warp waited for a free accumulator", 84: "4-bit product of many tokens: the unpacking waited for weights or for room",
+                85: "4-bit product of many tokens: the sums waited for weights or an accumulator",
                 20: "decode attention: a wait for a stage of keys and values"}
 
 

@@ -1,4 +1,4 @@
-"""Weights of 4 bits: making them, and products with them (`csrc/gemm_q4.cu`, `csrc/gemm_q4_pair.cu`, `csrc/gemv_q4.cu`, `csrc/quantize_q4.cu`).
+"""Weights of 4 bits: making them, and products with them (`csrc/gemm_q4.cu`, `csrc/gemm_q4_long.cu`, `csrc/gemv_q4.cu`, `csrc/quantize_q4.cu`).
 
     w[n, k] = scale[n, k // group] * (code[n, k] - zero[n, k // group])
 
@@ -24,7 +24,7 @@ from .ops import KernelError, _check, _stream, device_status
 
 _P, _I, _F, _L = ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_longlong
 
-SOURCES = ["gemm_q4.cu", "gemm_q4_pair.cu", "gemv_q4.cu", "quantize_q4.cu"]
+SOURCES = ["gemm_q4.cu", "gemm_q4_long.cu", "gemv_q4.cu", "quantize_q4.cu"]
 _SIGNATURES = {
     "tl_q4_block_bytes": [_I, _I, _I],
     "tl_gemm_q4": [_P, _L, _P, _P, _I, _I, _I, _I, _I, _F, _F, _P, _P],

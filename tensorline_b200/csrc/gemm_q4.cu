@@ -18,16 +18,14 @@ int gemm_q4_long(const Q4Args& G, int bn, cudaStream_t stream);     // gemm_q4_l
 
 namespace {
 
+constexpr int QG_THREADS = 320;                          // warp 0: copies, 1: tensor memory + products, 2..5: unpacking, 6..9: sums
 constexpr int QG_STAGES_MAX = 12;
 
 template <int BN> struct QgShape {
     static constexpr int X_HALF = BN * 128, X_BYTES = 2 * X_HALF;         // BN tokens x 64 k, twice
-    static constexpr int NA = BN <= 16 ? 3 : BN <= 64 ? 2 : 4;            // unpacked blocks in turn, 64 columns each
+    static constexpr int NA = BN <= 64 ? 2 : 4;                           // unpacked blocks in turn, 64 columns each
     static constexpr int ND = BN <= 32 ? 4 : 2;                           // groups' sums in turn
     static constexpr int PER_SM = BN <= 64 ? 2 : 1;
-    static constexpr int UG = 1;                                          // groups of four unpacking warps, a block of k each in turn
-    static constexpr int SUMS = 2 + 4 * UG;                               // warp 0: copies, 1: tensor memory + products, 2..: unpacking, SUMS..: sums
-    static constexpr int THREADS = 32 * (SUMS + 4);
     static constexpr uint32_t COLS = BN <= 64 ? 256 : 512;
     static constexpr int D_COL = NA * 64;
     static constexpr int SMEM_MOST = PER_SM == 2 ? 112 * 1024 : 226 * 1024;
@@ -35,7 +33,7 @@ template <int BN> struct QgShape {
 };
 
 template <int BN, int GROUP, bool ZEROS>
-__global__ void __launch_bounds__(QgShape<BN>::THREADS, QgShape<BN>::PER_SM)
+__global__ void __launch_bounds__(QG_THREADS, QgShape<BN>::PER_SM)
 gemm_q4_kernel(const __grid_constant__ CUtensorMap map_x, const Q4Args G) {
     using Sh = QgShape<BN>;
     constexpr int NA = Sh::NA, ND = Sh::ND, GROUPS = Q4_K / GROUP;
@@ -110,7 +108,7 @@ gemm_q4_kernel(const __grid_constant__ CUtensorMap map_x, const Q4Args G) {
         constexpr uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(Q4_ROWS >> 4) << 24);
         const uint32_t one = q4_elect();
         grid_dependency_wait();                          // the bounded waits start counting once the tokens can land
-        int d = 0, s = 0, turn = 0;
+        int d = 0, s = 0;
         bool ok = true;
         for (int i = 0; i < n_k && ok; ++i) {
             const int b = i % NA;
@@ -135,17 +133,15 @@ gemm_q4_kernel(const __grid_constant__ CUtensorMap map_x, const Q4Args G) {
                 ++d;
             }
             if (!ok) break;
-            if (++s == S) { s = 0; ++turn; }
+            if (++s == S) s = 0;
         }
-    } else if (warp < Sh::SUMS) {
+    } else if (warp < 6) {
         // ---------------------------------------------------------------- unpacking
         const int row = quarter * 32 + lane, zeros_at = Q4_CODES + G.form.groups * Q4_ROWS * (G.form.scale_f32 ? 4 : 2);
-        if (!G.at_rest) grid_dependency_wait();
+        grid_dependency_wait();                          // as above
         const uint32_t magic = q4_magic();
-        int i = (warp - 2) >> 2, s = i, turn = 0;
-        for (; i < n_k; i += Sh::UG) {
+        for (int i = 0, s = 0, turn = 0; i < n_k; ++i) {
             const int b = i % NA;
-            while (s >= S) { s -= S; ++turn; }
             if (!q4_wait(full + 8 * s, turn & 1, abort_flag, G.status, 74)) break;
             const uint32_t st = ring + s * G.stage_bytes + Sh::X_BYTES;
             uint4 q[4];
@@ -179,7 +175,7 @@ gemm_q4_kernel(const __grid_constant__ CUtensorMap map_x, const Q4Args G) {
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             __syncwarp();
             if (lane == 0) q4_arrive(a_full + 8 * b);
-            s += Sh::UG;
+            if (++s == S) { s = 0; ++turn; }
         }
     } else {
         // ---------------------------------------------------------------- sums
@@ -238,7 +234,7 @@ gemm_q4_kernel(const __grid_constant__ CUtensorMap map_x, const Q4Args G) {
     }
     if (nz > 1 || G.gate) {
         if (nz > 1) pair_cluster_sync(); else __syncthreads();
-        if (warp >= 2 && !*abort_flag) q4_finish<1, BN>(G, red, tile, t0, nz, blockIdx.z, (int)threadIdx.x - 64, Sh::THREADS - 64);
+        if (warp >= 2 && !*abort_flag) q4_finish<1, BN>(G, red, tile, t0, nz, blockIdx.z, (int)threadIdx.x - 64, QG_THREADS - 64);
         if (nz > 1) pair_cluster_sync();                 // nobody leaves while its shared memory is read
     }
     // -------------------------------------------------------------------- teardown
@@ -264,13 +260,12 @@ int qg_launch(const CUtensorMap& map, Q4Args G, int tiles, int splits, cudaStrea
     G.stage_bytes = (Sh::X_BYTES + G.form.bytes + 1023) & ~1023;
     G.stages = (Sh::SMEM_MOST - 1024 - BARS) / G.stage_bytes;
     if (G.stages > QG_STAGES_MAX) G.stages = QG_STAGES_MAX;
-    G.stages &= ~(Sh::UG - 1);                           // a stage belongs to one group of unpacking warps: none waits for a phase two ahead
     if (G.stages > G.per) G.stages = G.per;
     size_t ring = (size_t)G.stages * G.stage_bytes;      // it holds the sums, [BN][128] floats, in the end
     if (ring < (size_t)BN * Q4_ROWS * 4) { G.stages = (int)(((size_t)BN * Q4_ROWS * 4 + G.stage_bytes - 1) / G.stage_bytes); ring = (size_t)G.stages * G.stage_bytes; }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(tiles, (G.T + BN - 1) / BN, splits);
-    cfg.blockDim = dim3(Sh::THREADS);
+    cfg.blockDim = dim3(QG_THREADS);
     cfg.dynamicSmemBytes = ring + 1024 + BARS;
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
@@ -331,11 +326,11 @@ TL_EXPORT int tl_q4_block_bytes(int group, int scale_f32, int zeros) {
 // gate, y is float, no kernel of this stream that could still be running writes the weights.  Gate 1..3: rows of w are gates and what they
 // weigh, alternating in blocks of 64 (N % 128 == 0), and y [T, N / 2] is act(gate) * up: 1 silu, 2 the tanh form of gelu, 3 the clamped
 // swish with `limit` and `alpha`.  Returns 0, a CUDA error or 1 for what it does not take.
-TL_EXPORT int tl_gemm_q4(const void* x, long long ldx, const void* w, void* y, int ldo, int T, int N, int K, int form, float limit, float alpha,
+TL_EXPORT int tl_gemm_q4(const void* x, long long ldx, const void* w, void* y, long long ldo, int T, int N, int K, int form, float limit, float alpha,
                          int* status, cudaStream_t stream) {
     Q4Args G{};
     const int gate = form >> 10 & 3, out_f32 = form >> 12 & 1;
-    if (form < 0 || form >> 14 || T < 0 || N < 1 || K < 1 || (K & 7) || !q4_form(&G.form, form & 255, form >> 8 & 1, form >> 9 & 1)) return 1;
+    if (form < 0 || form >> 14 || T < 0 || T > Q4_MOST || N < 1 || N > Q4_MOST || K < 1 || K > Q4_MOST || (K & 7) || !q4_form(&G.form, form & 255, form >> 8 & 1, form >> 9 & 1)) return 1;
     if ((gate && (N & 127)) || ldo < (gate ? N / 2 : N)) return 1;
     if (T == 0) return 0;
     if (ldx < K || (ldx & 7) || ((uintptr_t)x & 15) || ((uintptr_t)w & 15) || !y || !status) return 1;
@@ -348,9 +343,8 @@ TL_EXPORT int tl_gemm_q4(const void* x, long long ldx, const void* w, void* y, i
     if (T <= Q4_FEW) return gemv_q4(G, stream);
     if (T > 64)
         if (const int tokens = qg_tile_tokens(T, N, G.blocks)) return gemm_q4_long(G, tokens, stream);
-    const int bn = T <= 16 ? 16 : T <= 32 ? 32 : T <= 64 ? 64 : 128;
+    const int bn = T <= 32 ? 32 : T <= 64 ? 64 : 128;
     const int tiles = (N + Q4_ROWS - 1) / Q4_ROWS, t_tiles = (T + bn - 1) / bn;
-    if (t_tiles > 65535) return 1;
     const int room = tl_num_sms() * (bn <= 64 ? 2 : 1);
     const long long work = (long long)tiles * t_tiles;
     int splits = work < room ? (int)(room / work) : 1;
@@ -361,7 +355,6 @@ TL_EXPORT int tl_gemm_q4(const void* x, long long ldx, const void* w, void* y, i
     CUtensorMap map;
     if ((e = q4_map(&map, x, T, K, ldx, bn, 64))) return e;
     switch (bn) {
-        case 16: return qg_launch_form<16>(map, G, tiles, splits, stream);
         case 32: return qg_launch_form<32>(map, G, tiles, splits, stream);
         case 64: return qg_launch_form<64>(map, G, tiles, splits, stream);
         default: return qg_launch_form<128>(map, G, tiles, splits, stream);

@@ -18,7 +18,7 @@ constexpr int QL_REGS_COPY = 56, QL_REGS_UNPACK = 80, QL_REGS_SUM = 128;
 static_assert(QL_REGS_COPY + 2 * QL_REGS_UNPACK + 2 * QL_REGS_SUM <= 5 * 96, "a larger share would be waited for without end");
 constexpr int QL_MOST = 128, QL_CW = QL_MOST / 2;        // tokens of a tile, of a summing warp
 constexpr int QL_NA = 4, QL_ND = 2, QL_D_COL = QL_NA * 64;      // unpacked blocks of k in turn (64 columns), groups' sums in turn
-constexpr int QL_STAGES_MAX = 12, QL_SMEM = 226 * 1024, QL_HAND = 2 * 2 * 16 * 64 * 4;      // gates and what they weigh change places: [2][half][16][64]
+constexpr int QL_STAGES_MAX = 12, QL_SMEM = 226 * 1024, QL_HAND = 2 * 2 * 16 * 64 * 4;      // gates and what they weigh change places: [in turn: 2][half][16][64]
 static_assert(QL_D_COL + QL_ND * QL_MOST <= 512, "tensor memory");
 
 struct QlArgs { Q4Args g; int bn, m_tiles, t_tiles; };
@@ -41,6 +41,7 @@ gemm_q4_long_kernel(const __grid_constant__ CUtensorMap map_x, const QlArgs A) {
     const uint32_t a_empty = a_full + 8 * NA;            // [NA] the products
     const uint32_t d_full = a_empty + 8 * NA;            // [ND] the products
     const uint32_t d_empty = d_full + 8 * ND;            // [ND] 8 summing warps
+    const uint32_t handed = d_empty + 8 * ND;            // [2] the 4 summing warps of a half
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int first = blockIdx.x, step = gridDim.x, items = A.m_tiles * A.t_tiles, n_k = G.blocks;
@@ -50,6 +51,7 @@ gemm_q4_long_kernel(const __grid_constant__ CUtensorMap map_x, const QlArgs A) {
         for (int s = 0; s < S; ++s) { q4_init(full + 8 * s, 1); q4_init(empty + 8 * s, 12); }
         for (int b = 0; b < NA; ++b) { q4_init(a_full + 8 * b, 4); q4_init(a_empty + 8 * b, 1); }
         for (int b = 0; b < ND; ++b) { q4_init(d_full + 8 * b, 1); q4_init(d_empty + 8 * b, 8); }
+        for (int h = 0; h < 2; ++h) q4_init(handed + 8 * h, 4);
         abort_word = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -146,7 +148,7 @@ gemm_q4_long_kernel(const __grid_constant__ CUtensorMap map_x, const QlArgs A) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(QL_REGS_UNPACK));
         const int row = quarter * 32 + lane, zeros_at = Q4_CODES + GROUPS * Q4_ROWS * (G.form.scale_f32 ? 4 : 2);
         const uint32_t magic = q4_magic();
-        if (!G.at_rest) grid_dependency_wait();
+        grid_dependency_wait();                          // as above
         const int mine = (warp - 4) >> 2;
         const int blocks = ((items - first + step - 1) / step) * n_k;                    // of k, of all of its tiles
         int s = mine, turn = 0;
@@ -190,7 +192,7 @@ gemm_q4_long_kernel(const __grid_constant__ CUtensorMap map_x, const QlArgs A) {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(QL_REGS_SUM));
         const int row = quarter * 32 + lane, half = (warp - 12) >> 2, cw = BN / 2;
         grid_dependency_wait();                          // the output may still be read by the kernel in front
-        int s = 0, d = 0;
+        int s = 0, d = 0, hands = 0;                     // times that values changed places
         bool ok = true;
         for (int item = first; item < items && ok; item += step) {
             float acc[QL_CW];
@@ -243,16 +245,20 @@ gemm_q4_long_kernel(const __grid_constant__ CUtensorMap map_x, const QlArgs A) {
                 }
             } else {
                 // Gates are rows 0..63 of a tile and lie in other warps than what they weigh: of 16 tokens at a time the one side hands over its
-                // values of the first eight, the other of the second, and each finishes eight.
+                // values of the first eight, the other of the second, and each finishes eight.  (Two buffers in turn: whoever writes one again has
+                // waited for the hand-over in between, which nobody makes before it has read the one.)
                 const bool up = quarter >= 2;
                 const int f = (quarter & 1) * 32 + lane, n = tile * 64 + f;
 #pragma unroll
                 for (int c0 = 0; c0 < QL_CW; c0 += 16) {
-                    if (c0 >= cw) break;
-                    float* h = hand + (((c0 >> 4) & 1) * 2 + half) * 16 * 64;
+                    if (c0 >= cw || !ok) break;
+                    float* h = hand + ((hands & 1) * 2 + half) * 16 * 64;
 #pragma unroll
                     for (int j = 0; j < 8; ++j) h[(up ? j : 8 + j) * 64 + f] = up ? acc[c0 + j] : acc[c0 + 8 + j];
-                    if (half) asm volatile("bar.sync 2, 128;" ::: "memory"); else asm volatile("bar.sync 1, 128;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0) q4_arrive(handed + 8 * half);
+                    if (!q4_wait(handed + 8 * half, hands & 1, abort_flag, G.status, 86)) { ok = false; break; }
+                    ++hands;
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
                         const int t = t0 + c0 + (up ? 8 : 0) + j;
@@ -290,7 +296,7 @@ int ql_launch(const CUtensorMap& map, const QlArgs& A, int blocks, cudaStream_t 
 // The product of G.T tokens in tiles of `bn` (a multiple of 32, at most 128); `G` is filled in but for the ring (gemm_q4.cu).
 int gemm_q4_long(const Q4Args& G, int bn, cudaStream_t stream) {
     QlArgs A{G, bn, (G.N + Q4_ROWS - 1) / Q4_ROWS, (G.T + bn - 1) / bn};
-    constexpr int BARS = (2 * QL_STAGES_MAX + 2 * QL_NA + 2 * QL_ND) * 8 + 16;
+    constexpr int BARS = (2 * QL_STAGES_MAX + 2 * QL_NA + 2 * QL_ND + 2) * 8;
     A.g.stage_bytes = (bn * 256 + G.form.bytes + 1023) & ~1023;
     A.g.stages = (QL_SMEM - 1024 - QL_HAND - BARS) / A.g.stage_bytes;
     if (A.g.stages > QL_STAGES_MAX) A.g.stages = QL_STAGES_MAX;

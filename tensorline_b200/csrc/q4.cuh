@@ -16,7 +16,7 @@ struct Q4Form { int group, groups, scale_f32, zeros, bytes; };      // k a group
 struct Q4Args {
     const unsigned char* x; long long ldx;               // tokens, bfloat16, rows `ldx` values apart
     const unsigned char* w; int blocks;                  // packed weights; blocks of k a tile of rows has
-    void* out; int out_f32, ldo;
+    void* out; long long ldo; int out_f32;
     int N, K, T;
     Q4Form form;
     int per;                                             // blocks of k a range (grid z)
@@ -29,6 +29,7 @@ struct Q4Args {
 namespace {
 
 constexpr int Q4_ROWS = 128, Q4_K = 128, Q4_CODES = Q4_ROWS * Q4_K / 2;
+constexpr int Q4_MOST = 0x7fffff00;                       // tokens, rows and columns: a tile's end is still an int
 constexpr int Q4_FEW = 16;                                // tokens up to which gemv_q4.cu takes a product
 
 // 0 if there is no such form

@@ -183,13 +183,13 @@ STATUS_ROLES = {1: "tcgen05 product: the copy thread waited for a free stage", 2
                 63: "matrix memory's outputs: the MMA warp waited for a stage", 64: "matrix memory's outputs: the workers waited for Q K",
                 65: "matrix memory's outputs: the workers waited for a sum", 66: "matrix memory's end states: the MMA warp waited for a free accumulator",
                 67: "matrix memory's outputs: the MMA warp waited for free accumulators",
-                71: "4-bit product: the copy thread waited for a free stage", 72: "4-bit product: the MMA warp waited for tokens or unpacked weights",
+                71: "4-bit product: the copy thread waited for a free stage", 72: "4-bit product: the MMA warp waited for unpacked weights",
                 73: "4-bit product: the MMA warp waited for a free accumulator", 74: "4-bit product: the unpacking waited for weights or for room",
-                75: "4-bit product: the sums waited for weights or an accumulator",
+                75: "4-bit product: the sums waited for an accumulator",
                 76: "4-bit product of few tokens: the copy thread waited for a free stage", 77: "4-bit product of few tokens: a warp waited for a stage's copies",
-                81: "4-bit product of many tokens: a copy thread waited for a free stage", 82: "4-bit product of many tokens: the MMA warp waited for tokens or weights",
+                81: "4-bit product of many tokens: a copy thread waited for a free stage", 82: "4-bit product of many tokens: the MMA warp waited for unpacked weights",
                 83: "4-bit product of many tokens: the MMA warp waited for a free accumulator", 84: "4-bit product of many tokens: the unpacking waited for weights or for room",
-                85: "4-bit product of many tokens: the sums waited for weights or an accumulator",
+                85: "4-bit product of many tokens: the sums waited for an accumulator", 86: "4-bit product of many tokens: gates waited for what they weigh",
                 20: "decode attention: a wait for a stage of keys and values"}
 
 

@@ -27,13 +27,15 @@ _P, _I, _F, _L = ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_longlon
 SOURCES = ["gemm_q4.cu", "gemm_q4_long.cu", "gemv_q4.cu", "quantize_q4.cu"]
 _SIGNATURES = {
     "tl_q4_block_bytes": [_I, _I, _I],
-    "tl_gemm_q4": [_P, _L, _P, _P, _I, _I, _I, _I, _I, _F, _F, _P, _P],
+    "tl_gemm_q4": [_P, _L, _P, _P, _L, _I, _I, _I, _I, _F, _F, _P, _P],
     "tl_quantize_q4": [_P, _I, _P, _I, _I, _I, _P],
     "tl_dequantize_q4": [_P, _P, _I, _I, _I, _I, _P],
 }
 GROUPS = (32, 64, 128)
 ROWS = K_BLOCK = 128                                      # of a stored block
 CODE_BYTES = ROWS * K_BLOCK // 2
+MOST = 0x7fffff00                                         # tokens, rows and columns
+MOST_ROWS = 65535 * ROWS                                  # of a matrix that is quantized or read back
 _lib = None
 
 
@@ -75,8 +77,8 @@ class Q4Weight:
     def __init__(self, data: torch.Tensor, n: int, k: int, group: int = 128, zeros: bool = False, scale_dtype: torch.dtype = torch.bfloat16,
                  at_rest: bool = False):
         want = (-(-n // ROWS), -(-k // K_BLOCK), block_bytes(group, scale_dtype, zeros))
-        if n < 1 or k < 1 or k % 8:
-            raise KernelError(f"4-bit weights [{n}, {k}]: the sizes are positive and the second a multiple of 8")
+        if not 1 <= n <= MOST or not 1 <= k <= MOST or k % 8:
+            raise KernelError(f"4-bit weights [{n}, {k}]: the sizes are 1 to {MOST} and the second a multiple of 8")
         if data.dtype is not torch.uint8 or data.shape != want or not data.is_contiguous():
             raise KernelError(f"4-bit weights [{n}, {k}] in groups of {group} are a contiguous uint8 {list(want)}, "
                               f"not {data.dtype} {list(data.shape)}")
@@ -130,8 +132,8 @@ def quantize(w: torch.Tensor, group: int = 128, zeros: bool = False, scale_dtype
         raise KernelError(f"quantize takes a contiguous bfloat16 or float32 matrix, not {w.dtype} {list(w.shape)}")
     index, (n, k) = _device(w), w.shape
     size = block_bytes(group, scale_dtype, zeros)
-    if n < 1 or k < 1 or k % 8 or w.data_ptr() % 16:
-        raise KernelError(f"quantize: [{n}, {k}] needs positive sizes, the second a multiple of 8, and a base on a 16-byte boundary")
+    if not 1 <= n <= MOST_ROWS or not 1 <= k <= MOST or k % 8 or w.data_ptr() % 16:
+        raise KernelError(f"quantize: [{n}, {k}] needs 1 to {MOST_ROWS} rows, a multiple of 8 columns and a base on a 16-byte boundary")
     if (other := _on(index)) is not None:
         with other:
             return quantize(w, group, zeros, scale_dtype)
@@ -144,6 +146,8 @@ def dequantize(w: Q4Weight, dtype: torch.dtype = torch.float32) -> torch.Tensor:
     """The values that `w` stands for, [N, K]: float32, or those rounded to bfloat16."""
     if dtype not in (torch.bfloat16, torch.float32):
         raise KernelError(f"dequantize gives bfloat16 or float32, not {dtype}")
+    if w.n > MOST_ROWS:
+        raise KernelError(f"dequantize: {w.n} rows are more than {MOST_ROWS}")
     if (other := _on(_device(w.data))) is not None:
         with other:
             return dequantize(w, dtype)
@@ -196,9 +200,9 @@ _status: dict = {}                                        # device index -> addr
 def _gate(gated):
     """`gated` as the C entry takes it: (bits, limit, alpha)."""
     if isinstance(gated, tuple):
-        if len(gated) == 3 and gated[0] == "swish_clamped" and gated[1] > 0:
+        if len(gated) == 3 and gated[0] == "swish_clamped" and all(isinstance(v, (int, float)) for v in gated[1:]) and gated[1] > 0:
             return 3 << 10, float(gated[1]), float(gated[2])
-    elif gated in _GATES:
+    elif isinstance(gated, (str, bool)) and gated in _GATES:
         return _GATES[gated], 0.0, 1.0
     raise KernelError(f"a gated epilogue applies 'silu', 'gelu_tanh' or ('swish_clamped', limit, alpha), not {gated!r}")
 
@@ -220,8 +224,8 @@ def gemm_q4(x: torch.Tensor, w: Q4Weight, out_dtype: torch.dtype = torch.bfloat1
             raise KernelError(f"gemm_q4: gate and up rows alternate in blocks of 64, {n} rows are no multiple of 128")
     cols = n // 2 if gated else n
     shape = x.shape
-    if x.dtype is not torch.bfloat16 or len(shape) != 2 or shape[1] != k:
-        raise KernelError(f"gemm_q4: x is bfloat16 [T, {k}], not {x.dtype} {list(shape)}")
+    if x.dtype is not torch.bfloat16 or len(shape) != 2 or shape[1] != k or shape[0] > MOST:
+        raise KernelError(f"gemm_q4: x is bfloat16 [T, {k}] of at most {MOST} tokens, not {x.dtype} {list(shape)}")
     if out_dtype is torch.float32:
         form |= _OUT_F32
     elif out_dtype is not torch.bfloat16:
@@ -240,7 +244,7 @@ def gemm_q4(x: torch.Tensor, w: Q4Weight, out_dtype: torch.dtype = torch.bfloat1
         raise KernelError("gemm_q4: x has unit inner stride and rows that start on 16-byte boundaries, one behind the other")
     ldo = cols
     if out is None:
-        out = x.new_empty((T, cols), dtype=out_dtype)
+        out = torch.empty_strided((T, cols), (cols, 1), dtype=out_dtype, device=x.device)
     else:
         if T > 1:
             ldo = out.stride(0)

@@ -54,11 +54,22 @@ def test_no_path_on_the_host():
 @pytest.mark.parametrize("x,more", [
     (torch.zeros(2, 64), {}), (torch.zeros(2, 72, dtype=torch.bfloat16), {}), (torch.zeros(64, dtype=torch.bfloat16), {}),
     (torch.zeros(2, 64, dtype=torch.bfloat16), dict(out_dtype=torch.float16)), (torch.zeros(2, 64, dtype=torch.bfloat16), dict(gated="relu")),
-    (torch.zeros(2, 64, dtype=torch.bfloat16), dict(gated=("swish_clamped", 0.0, 1.0))), (torch.zeros(2, 64, dtype=torch.bfloat16), dict(gated="silu"))])
+    (torch.zeros(2, 64, dtype=torch.bfloat16), dict(gated=("swish_clamped", 0.0, 1.0))), (torch.zeros(2, 64, dtype=torch.bfloat16), dict(gated="silu")),
+    (torch.zeros(2, 64, dtype=torch.bfloat16), dict(gated=["silu"])), (torch.zeros(2, 64, dtype=torch.bfloat16), dict(gated=("swish_clamped", "7", 1.0)))])
 def test_refused_products(x, more):
     w = ops_q4.pack(torch.zeros(4, 64, dtype=torch.int64), torch.ones(4, 1))
     with pytest.raises(KernelError):
         ops_q4.gemm_q4(x, w, **more)
+
+
+def test_sizes_that_the_entries_have_no_room_for():
+    w = ops_q4.pack(torch.zeros(4, 64, dtype=torch.int64), torch.ones(4, 1))
+    with pytest.raises(KernelError, match="at most"):
+        ops_q4.gemm_q4(torch.empty(2 ** 32 + 1, 64, dtype=torch.bfloat16, device="meta"), w)
+    with pytest.raises(KernelError, match="rows"):
+        ops_q4.dequantize(ops_q4.Q4Weight(torch.empty(65536, 1, 8448, dtype=torch.uint8, device="meta"), 65536 * 128, 128))
+    with pytest.raises(KernelError, match="sizes"):
+        ops_q4.Q4Weight(torch.empty(2 ** 25, 1, 8448, dtype=torch.uint8, device="meta"), 2 ** 32, 128)
 
 
 def test_entries_are_declared_as_they_are_called():
@@ -89,7 +100,7 @@ def test_c_entries_refuse_what_they_do_not_take():
     """No pointer is looked at before the sizes: these end on the host."""
     lib, p = ops_q4.lib(), 1 << 20
     good = dict(x=p, ldx=64, w=p, y=p, ldo=128, T=2, N=128, K=64, form=64, limit=0.0, alpha=1.0, status=p, stream=None)
-    for bad in (dict(T=-1), dict(N=0), dict(K=0), dict(K=60), dict(form=16), dict(form=64 | 1 << 14), dict(form=-1), dict(form=64 | 1 << 10, N=192),
+    for bad in (dict(T=-1), dict(T=0x7fffff01), dict(N=0x7fffff01, ldo=1 << 31), dict(K=0x7fffff08, ldx=1 << 31), dict(N=0), dict(K=0), dict(K=60), dict(form=16), dict(form=64 | 1 << 14), dict(form=-1), dict(form=64 | 1 << 10, N=192),
                 dict(ldo=100), dict(ldx=56), dict(ldx=68), dict(x=p + 2), dict(w=p + 8), dict(y=None), dict(status=None)):
         assert lib.tl_gemm_q4(*{**good, **bad}.values()) == 1, bad
     assert lib.tl_gemm_q4(*{**good, "T": 0}.values()) == 0

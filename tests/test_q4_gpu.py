@@ -167,6 +167,20 @@ def test_gates(q4, gated, T, n, k):
         assert bool(((got.double() - want).abs() <= (slope + own) * 1.01 + (want.abs() * 2.0 ** -8 if out is BF else 0)).all())
 
 
+def test_gates_of_short_sums_tile_after_tile(q4):
+    """Several tiles a block, whose sums are one or two groups: what changes places for one tile is read before the next one's is written."""
+    for k, group in ((64, 64), (128, 64), (128, 128)):
+        w, values_ = whole(q4, 600 * 64, k, group, False, F32)
+        x = whole_x(192, k)
+        sums = (x.double() @ values_.T).view(192, 300, 2, 64)
+        got = q4.gemm_q4(x, w, F32, gated="silu").double()
+        want = gates(sums[:, :, 0].reshape(192, -1), sums[:, :, 1].reshape(192, -1), "silu")
+        # Exact sums.  In halves of 2^-23: an exponential e (4), times its share of 1 + e in the reciprocal of that (2), the sum, the reciprocal and
+        # three products: 11.  Exponentials below the smallest normal float, 2^-126, weigh sums of less than 2^13.
+        assert ((got - want).abs() <= 12 * 2.0 ** -24 * want.abs() + 2.0 ** -100).all()
+        assert torch.equal(got, q4.gemm_q4(x, w, F32, gated="silu").double())
+
+
 def test_far_gates(q4):
     """Gates whose exponential is no float any more: the quotient is small or nothing, never a number that is none."""
     a = torch.tensor([-1e4, -200.0, -100.0, -88.0, 0.0, 88.0, 200.0, 1e4])
@@ -232,6 +246,21 @@ def test_rows_that_lie_apart(q4, T, gated):
         assert torch.equal(got.double(), x.double() @ m.t())
     room[1:T + 1, 3:n + 3] = 5.0
     assert bool((room == 5.0).all())
+
+
+@pytest.mark.parametrize("T,gated", [(2, False), (2, "silu"), (40, False), (130, "silu")])
+def test_rows_more_than_31_bits_apart(q4, T, gated):
+    far = 2 ** 31 + 8 if T == 2 else 2 ** 31 // 32
+    w, _ = whole(q4, 256, 128, 64, False, BF)
+    x = whole_x(T, 128)
+    cols = 128 if gated else 256
+    room = torch.empty((T - 1) * far + 256, dtype=BF, device="cuda")
+    wide = room.as_strided((T, cols), (far, 1))
+    assert q4.gemm_q4(x, w, gated=gated, out=wide) is wide
+    assert torch.equal(wide, q4.gemm_q4(x, w, gated=gated))
+    tokens = room.as_strided((T, 128), (far, 1))
+    tokens.copy_(x)
+    assert torch.equal(q4.gemm_q4(tokens, w, gated=gated), q4.gemm_q4(x, w, gated=gated))
 
 
 def test_refusals(q4):

@@ -293,25 +293,71 @@ int qg_launch_form(const CUtensorMap& map, const Q4Args& G, int tiles, int split
            G.form.group == 64 ? qg_launch<BN, 64, false>(map, G, tiles, splits, stream) : qg_launch<BN, 32, false>(map, G, tiles, splits, stream);
 }
 
-// Tokens of a tile of gemm_q4_long.cu, 0: ranges of K in clusters (this file) are faster.  Its blocks, one a SM, take a block of k through in about
-// 370 + 1.1 ns a token (measured 410, 434, 480 and 510 ns at 32, 64, 96 and 128 tokens), so it is the tile with which they are done first.
-// With fewer tiles than half of the SMs, ranges of K in clusters may be done before it: a block of k 540 ns there and 13 us for the rest.  Measured,
-// us, here / there:  128 tokens, 28 tiles x 148 blocks of k 44 / 65;  74 x 28 22.5 / 17.9;  256 tokens, 28 x 148 50 / 68;  200 tokens, 36 x 28 21.3 / 17.5.
-int qg_tile_tokens(int T, int N, int blocks) {
-    const int sms = tl_num_sms(), m_tiles = (N + Q4_ROWS - 1) / Q4_ROWS;
-    int best = 0;
-    long long least = 0;                                 // tenths of ns
-    for (int bn = 128; bn >= 32; bn -= 32) {
-        const long long items = (long long)m_tiles * ((T + bn - 1) / bn), rounds = (items + sms - 1) / sms;
-        const long long cost = rounds * blocks * (3700 + 11 * bn) + 40000;
-        if (!best || cost < least) { best = bn; least = cost; }
+// How a product's tokens are gone through, and about how long that takes.
+struct QgPlan { int bn, long_, splits, first; double us; };      // tokens of a tile; of gemm_q4_long.cu?; ranges of K; tokens before the rest is planned anew
+
+// Ranges of K in clusters, for one launch over `tiles` of `bn` tokens.  An SM that has two thread blocks takes 1.4 times as long for a block of k of
+// each; of 148 SMs about 133 get a block in clusters of two or three, 118 in clusters of four and 98 in larger ones (of two a SM 266, of seven and
+// more 252), and clusters that find no room begin when others have ended.  Measured at 1, 2 .. 8 ranges, us:  45 tokens, 40 tiles x 108 blocks of k
+// 57 33 24 25 22 19 28 26;  64, 28 x 148: 77 44 31 25 27 24 23 20;  64, 216 x 40: 37 38 47 48 50 56;  128, 28 x 148: 76 48 35 28 46 40 .. 34;
+// 90, 16 x 32: 21 18 14 11.4 10.6 10 .. 16.
+QgPlan qg_ranges(long long tiles, int blocks, int bn) {
+    const int sms = tl_num_sms(), two = bn <= 64;
+    QgPlan p{bn, 0, 1, 0, 0};
+    for (int s = 1; s <= 8 && s <= blocks; ++s) {
+        const int per = (blocks + s - 1) / s;
+        if ((blocks + per - 1) / per != s) continue;     // a range would be empty
+        const long long total = tiles * s, alone = s == 1 ? sms : s <= 3 ? sms * 9 / 10 : s == 4 ? sms * 4 / 5 : sms * 2 / 3;
+        const long long both = s == 1 ? 2 * sms : s <= 6 ? sms * 9 / 5 : sms * 17 / 10;
+        const double turns = total <= alone ? 1 : two ? 1.4 * ((total + both - 1) / both) : (total + alone - 1) / alone;
+        const double us = two ? turns * (per + 4) * (bn == 32 ? 0.5 : 0.6) + 2 : turns * (per * 0.55 + 10);
+        if (s == 1 || us < p.us) { p.splits = s; p.us = us; }
     }
-    const long long here = (long long)m_tiles * ((T + 127) / 128);
-    if (here * 2 <= sms) {
-        const long long ranges = sms / here < 8 ? sms / here : 8;
-        if ((blocks + ranges - 1) / ranges * 5400 + 130000 < least) return 0;
+    return p;
+}
+
+// One launch.  The blocks of gemm_q4_long.cu, one a SM, take a block of k through in 410, 420, 450 and 520 ns at 32, 64, 96 and 128 tokens: of its
+// tiles, the one with which they are done first.  Up to 64 tokens, and where there are so few tiles that many SMs would have none, ranges of K
+// in clusters are faster.  Measured, us, here / there:  128 tokens, 28 tiles x 148 blocks of k 28 / 65;  74 x 28 22 / 15.5;  256 tokens, 28 x 148 49 / 68.
+QgPlan qg_one(int T, int m_tiles, int blocks) {
+    const int here = T <= 32 ? 32 : T <= 64 ? 64 : 128, sms = tl_num_sms();
+    QgPlan p = qg_ranges((long long)m_tiles * ((T + here - 1) / here), blocks, here);
+    if (T > 64)
+        for (int bn = 128; bn >= 32; bn -= 32) {
+            const long long items = (long long)m_tiles * ((T + bn - 1) / bn), rounds = (items + sms - 1) / sms;
+            const double us = (double)rounds * blocks * (0.37 + 0.0011 * bn) + 3;
+            if (us < p.us) p = QgPlan{bn, 1, 0, 0, us};
+        }
+    return p;
+}
+
+// Many tokens leave SMs idle in their last round of tiles, nearly all of them at worst: the tokens of that round may be better off by themselves, in
+// tiles of another size or in ranges of K (2,048 tokens, 28 tiles of rows x 148 blocks of k: 448 tiles, three more than three rounds; 335 us at once).
+QgPlan qg_plan(int T, int m_tiles, int blocks) {
+    QgPlan p = qg_one(T, m_tiles, blocks);
+    for (int bn = 128; T > 128 && bn >= 64; bn -= 32) {
+        const int sms = tl_num_sms();
+        const long long rounds = ((long long)m_tiles * ((T + bn - 1) / bn) + sms - 1) / sms - 1;      // full ones
+        const long long first = rounds * sms / m_tiles * bn;
+        if (first <= 0 || first >= T) continue;
+        const double us = (double)rounds * blocks * (0.37 + 0.0011 * bn) + 5 + qg_one(T - (int)first, m_tiles, blocks).us;
+        if (us < p.us) p = QgPlan{bn, 1, 0, (int)first, us};
     }
-    return best;
+    return p;
+}
+
+int qg_run(Q4Args G, const QgPlan& p, cudaStream_t stream) {
+    if (p.long_) return gemm_q4_long(G, p.bn, stream);
+    const int tiles = (G.N + Q4_ROWS - 1) / Q4_ROWS;
+    G.per = (G.blocks + p.splits - 1) / p.splits;
+    CUtensorMap map;
+    const int e = q4_map(&map, G.x, G.T, G.K, G.ldx, p.bn, 64);
+    if (e) return e;
+    switch (p.bn) {
+        case 32: return qg_launch_form<32>(map, G, tiles, p.splits, stream);
+        case 64: return qg_launch_form<64>(map, G, tiles, p.splits, stream);
+        default: return qg_launch_form<128>(map, G, tiles, p.splits, stream);
+    }
 }
 
 }  // namespace
@@ -340,23 +386,16 @@ TL_EXPORT int tl_gemm_q4(const void* x, long long ldx, const void* w, void* y, l
     G.x = (const unsigned char*)x; G.ldx = ldx; G.w = (const unsigned char*)w; G.blocks = (K + Q4_K - 1) / Q4_K;
     G.out = y; G.out_f32 = out_f32; G.ldo = ldo; G.N = N; G.K = K; G.T = T;
     G.gate = gate; G.limit = limit; G.alpha = alpha; G.at_rest = at_rest; G.status = status;
-    if (T <= Q4_FEW) return gemv_q4(G, stream);
-    if (T > 64)
-        if (const int tokens = qg_tile_tokens(T, N, G.blocks)) return gemm_q4_long(G, tokens, stream);
-    const int bn = T <= 32 ? 32 : T <= 64 ? 64 : 128;
-    const int tiles = (N + Q4_ROWS - 1) / Q4_ROWS, t_tiles = (T + bn - 1) / bn;
-    const int room = tl_num_sms() * (bn <= 64 ? 2 : 1);
-    const long long work = (long long)tiles * t_tiles;
-    int splits = work < room ? (int)(room / work) : 1;
-    if (splits > 8) splits = 8;
-    if (splits > G.blocks) splits = G.blocks;
-    G.per = (G.blocks + splits - 1) / splits;
-    splits = (G.blocks + G.per - 1) / G.per;
-    CUtensorMap map;
-    if ((e = q4_map(&map, x, T, K, ldx, bn, 64))) return e;
-    switch (bn) {
-        case 32: return qg_launch_form<32>(map, G, tiles, splits, stream);
-        case 64: return qg_launch_form<64>(map, G, tiles, splits, stream);
-        default: return qg_launch_form<128>(map, G, tiles, splits, stream);
+    const int m_tiles = (N + Q4_ROWS - 1) / Q4_ROWS;
+    while (G.T > Q4_FEW) {
+        const QgPlan p = qg_plan(G.T, m_tiles, G.blocks);
+        if (!p.first) return qg_run(G, p, stream);
+        const int rest = G.T - p.first;
+        G.T = p.first;
+        if ((e = qg_run(G, p, stream))) return e;
+        G.T = rest;
+        G.x += (size_t)p.first * G.ldx * 2;
+        G.out = (unsigned char*)G.out + (size_t)p.first * G.ldo * (out_f32 ? 4 : 2);
     }
+    return gemv_q4(G, stream);
 }

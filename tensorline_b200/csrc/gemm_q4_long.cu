@@ -23,6 +23,52 @@ static_assert(QL_D_COL + QL_ND * QL_MOST <= 512, "tensor memory");
 
 struct QlArgs { Q4Args g; int bn, m_tiles, t_tiles; };
 
+// Half of a tile's tokens goes out, 32 rows a warp: `cw` of them, from t0 on.
+template <typename TY>
+__device__ __forceinline__ bool ql_tile_out(const Q4Args& G, const float (&acc)[QL_CW], int cw, int tile, int t0, int quarter, int lane, float* hand, uint32_t handed,
+                                            int& hands, volatile int* abort_flag) {
+    auto put = [](TY* at, float v) {
+        if constexpr (sizeof(TY) == 4) *at = v; else *at = __float2bfloat16_rn(v);
+    };
+    const int left = G.T - t0;                           // tokens that there are
+    if (!G.gate) {
+        const int n = tile * Q4_ROWS + quarter * 32 + lane, count = n < G.N ? left : 0;
+        TY* to = (TY*)G.out + t0 * G.ldo + n;
+#pragma unroll
+        for (int c0 = 0; c0 < QL_CW; c0 += 16) {
+            if (c0 >= cw) break;
+#pragma unroll
+            for (int c = c0; c < c0 + 16; ++c, to += G.ldo)
+                if (c < count) put(to, acc[c]);
+        }
+        return true;
+    }
+    // Gates are rows 0..63 of a tile and lie in other warps than what they weigh: of 16 tokens at a time the one side hands over its values of the
+    // first eight, the other of the second, and each finishes eight.  (Two buffers in turn: whoever writes one again has waited for the
+    // hand-over in between, which nobody makes before it has read the one.)
+    const bool up = quarter >= 2;
+    const int f = (quarter & 1) * 32 + lane, first = up ? 8 : 0;
+    TY* to = (TY*)G.out + (t0 + first) * G.ldo + tile * 64 + f;
+#pragma unroll
+    for (int c0 = 0; c0 < QL_CW; c0 += 16, to += 8 * G.ldo) {
+        if (c0 >= cw) break;
+        float* h = hand + (hands & 1) * (2 * 16 * 64) + f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) h[(up ? j : 8 + j) * 64] = up ? acc[c0 + j] : acc[c0 + 8 + j];
+        __syncwarp();
+        if (lane == 0) q4_arrive(handed);
+        if (!q4_wait(handed, hands & 1, abort_flag, G.status, 86)) return false;
+        ++hands;
+#pragma unroll
+        for (int j = 0; j < 8; ++j, to += G.ldo) {
+            const float mine = up ? acc[c0 + 8 + j] : acc[c0 + j], other = h[(first + j) * 64];
+            const float y = q4_gate(up ? other : mine, up ? mine : other, G.gate, G.limit, G.alpha);
+            if (c0 + first + j < left) put(to, y);
+        }
+    }
+    return true;
+}
+
 template <int GROUP, bool ZEROS>
 __global__ void __launch_bounds__(QL_THREADS, 1)
 gemm_q4_long_kernel(const __grid_constant__ CUtensorMap map_x, const QlArgs A) {
@@ -235,39 +281,9 @@ gemm_q4_long_kernel(const __grid_constant__ CUtensorMap map_x, const QlArgs A) {
             }
             if (!ok) break;
             const int tile = item / A.t_tiles, t0 = (item % A.t_tiles) * BN + half * cw;
-            if (!G.gate) {
-                const int n = tile * Q4_ROWS + row;
-                if (n < G.N) {
-                    const size_t base = (size_t)t0 * G.ldo + n;
-#pragma unroll
-                    for (int c = 0; c < QL_CW; ++c)
-                        if (c < cw && t0 + c < G.T) q4_store(G, base + (size_t)c * G.ldo, acc[c]);
-                }
-            } else {
-                // Gates are rows 0..63 of a tile and lie in other warps than what they weigh: of 16 tokens at a time the one side hands over its
-                // values of the first eight, the other of the second, and each finishes eight.  (Two buffers in turn: whoever writes one again has
-                // waited for the hand-over in between, which nobody makes before it has read the one.)
-                const bool up = quarter >= 2;
-                const int f = (quarter & 1) * 32 + lane, n = tile * 64 + f;
-#pragma unroll
-                for (int c0 = 0; c0 < QL_CW; c0 += 16) {
-                    if (c0 >= cw || !ok) break;
-                    float* h = hand + ((hands & 1) * 2 + half) * 16 * 64;
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) h[(up ? j : 8 + j) * 64 + f] = up ? acc[c0 + j] : acc[c0 + 8 + j];
-                    __syncwarp();
-                    if (lane == 0) q4_arrive(handed + 8 * half);
-                    if (!q4_wait(handed + 8 * half, hands & 1, abort_flag, G.status, 86)) { ok = false; break; }
-                    ++hands;
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        const int t = t0 + c0 + (up ? 8 : 0) + j;
-                        const float mine = up ? acc[c0 + 8 + j] : acc[c0 + j], other = h[((up ? 8 : 0) + j) * 64 + f];
-                        const float y = q4_gate(up ? other : mine, up ? mine : other, G.gate, G.limit, G.alpha);
-                        if (n < G.N / 2 && t < G.T) q4_store(G, (size_t)t * G.ldo + n, y);
-                    }
-                }
-            }
+            float* h = hand + half * (16 * 64);
+            if (G.out_f32) ok = ql_tile_out<float>(G, acc, cw, tile, t0, quarter, lane, h, handed + 8 * half, hands, abort_flag);
+            else ok = ql_tile_out<bf16>(G, acc, cw, tile, t0, quarter, lane, h, handed + 8 * half, hands, abort_flag);
         }
     }
     // -------------------------------------------------------------------- teardown

@@ -124,6 +124,28 @@ def test_whole_numbers_at_layer_sizes(q4, T, n, k):
     assert torch.equal(q4.gemm_q4(x, w, F32).double(), x.double() @ m.t())
 
 
+@pytest.mark.parametrize("T", [643, 700, 1284])
+@pytest.mark.parametrize("gated", [False, "silu"])
+def test_tokens_of_a_last_round_by_themselves(q4, T, gated):
+    """One or two full rounds of tiles and a few tokens more, which another kernel, or other tiles, take; rows that lie apart."""
+    n, k = 3584, 4096
+    w, values_ = whole(q4, n, k, 128, False, BF)
+    x = whole_x(T, k)
+    sums = x.double() @ values_.T
+    cols = n // 2 if gated else n
+    room = torch.full((T + 1, cols + 24), 7.0, dtype=F32, device="cuda")
+    wide = torch.zeros(T, k + 40, dtype=BF, device="cuda")
+    wide[:, :k] = x
+    q4.gemm_q4(wide[:, :k], w, F32, gated=gated, out=room[:T, :cols])
+    if gated:
+        sums = sums.view(T, n // 128, 2, 64)
+        want = gates(sums[:, :, 0].reshape(T, -1), sums[:, :, 1].reshape(T, -1), gated)
+        assert ((room[:T, :cols].double() - want).abs() <= 12 * 2.0 ** -24 * want.abs() + 2.0 ** -100).all()      # (test_gates_of_short_sums_tile_after_tile)
+    else:
+        assert torch.equal(room[:T, :cols].double(), sums)
+    assert (room[T:] == 7).all() and (room[:, cols:] == 7).all()
+
+
 @pytest.mark.parametrize("group,zeros,scale", FORMS)
 @pytest.mark.parametrize("T,n,k", [(3, 333, 2000), (40, 257, 3000), (130, 129, 1544), (1, 100, 18944)])
 def test_sums_in_float(q4, group, zeros, scale, T, n, k):

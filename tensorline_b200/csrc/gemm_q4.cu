@@ -10,6 +10,9 @@
 // which is where tcgen05.mma takes its 128-row operand from; one warp issues the products; four warps take a finished group's sums out of
 // tensor memory, scale and add them in registers.  Weights in tensor memory cost one store of 32 values a warp instead of a swizzled round
 // trip through shared memory, and their scale is one number a thread, since a row is a lane.
+// What bounds it: hand-overs between those warps, 540 ns a block of k at 64 tokens and 1.4 times that for two thread blocks an SM (unpacking alone 230,
+// the weights' way from memory 190).  Measured in a CUDA graph: 37,888 x 3,584 gated, 32 tokens 23 us, 64 tokens 29 us (floor 10.7); 3,584 x
+// 18,944, 64 tokens 20 us (5.3); 5,120 x 13,824 in groups of 64 with zeros and float scales, 45 tokens 23.5 us (6.4).
 // Every wait on a barrier is bounded: a block whose wait runs out records a code in `status`, stops and returns.
 #include "q4.cuh"
 
@@ -332,7 +335,8 @@ QgPlan qg_one(int T, int m_tiles, int blocks) {
 }
 
 // Many tokens leave SMs idle in their last round of tiles, nearly all of them at worst: the tokens of that round may be better off by themselves, in
-// tiles of another size or in ranges of K (2,048 tokens, 28 tiles of rows x 148 blocks of k: 448 tiles, three more than three rounds; 335 us at once).
+// tiles of another size or in ranges of K.  Measured, us, at once / so:  2,048 tokens, 28 tiles of rows x 148 blocks of k (448 tiles, four more than
+// three rounds take) 340 / 275;  700 tokens 136 / 100;  1,500 tokens, 40 x 108 239 / 206;  2,048 tokens, 1,188 x 28 2,245 / 1,985.
 QgPlan qg_plan(int T, int m_tiles, int blocks) {
     QgPlan p = qg_one(T, m_tiles, blocks);
     for (int bn = 128; T > 128 && bn >= 64; bn -= 32) {

@@ -7,8 +7,10 @@
 // rint: to the nearest whole number, ties to the even one.  A scale of zero leaves codes that stand for zeros; a group that holds a value that
 // is no number or infinite has a scale that is no number, so that whoever reads it sees it.
 //
-// Both kernels move a matrix once and are bound by that: a block of threads takes 128 rows and 128 k, 16 lanes a row, eight k a lane (one word
-// of codes).  Quotients are decided exactly without 64-bit arithmetic, see q4_rint.
+// Both kernels move a matrix once: a block of threads takes 128 rows and 128 k, 16 lanes a row, eight k a lane (one word of codes).  Reading back is
+// bound by that; making codes by its instructions, about 24 a value, although quotients are decided exactly without 64-bit arithmetic
+// (q4_round).  Measured, 37,888 x 3,584 in groups of 128: codes from bfloat16 123 us (floor 52), from float 145 (94); values in bfloat16 54 us
+// (52), in float 98 (94).
 #include "q4.cuh"
 
 namespace {

@@ -6,7 +6,8 @@ Options that both have keep the reference's names, meanings and defaults (server
 --model (or $TL_MODEL), --device, --dtype, --max-num-seqs, --max-batched-tokens, --num-blocks,
 --no-cuda-graphs, --no-overlap, --graph-warmup-tokens, --no-prefix-caching, --kv-cache-gb.
 Its server, quantization, speculation and multi-model options (--host, --port, --engine, --quant,
---spec-tokens, --serve, --gpu-budget-gb) have no counterpart and are refused by name.
+--spec-tokens, --serve, --gpu-budget-gb) have no counterpart under these names and are refused; weights
+of 4 bits are asked for with --weight-bits 4 (--weight-group, --weight-zeros, --quantize-head).
 
     tensorline --model DIR --prompt-ids 1,2,3 --max-tokens 16
     tensorline random-weights --config config.json --out DIR --seed 0

@@ -7,7 +7,7 @@
 //
 // A block works on 128 rows of W and BN tokens over a range of K, a block of 128 k at a time.  One warp brings the packed weights (one bulk copy a
 // block of k) and the tokens (by TMA, 128-byte swizzle) into a ring; four warps unpack the weights, a row a thread, straight into tensor memory,
-// which is where tcgen05.mma takes its 128-row operand from; one warp issues the products; four warps take a finished group's sums out of
+// which is where tcgen05.mma takes its 128-row operand from; one warp issues the products; four warps (eight at 128 tokens) take a finished group's sums out of
 // tensor memory, scale and add them in registers.  Weights in tensor memory cost one store of 32 values a warp instead of a swizzled round
 // trip through shared memory, and their scale is one number a thread, since a row is a lane.
 // What bounds it: hand-overs between those warps, 540 ns a block of k at 64 tokens and 1.4 times that for two thread blocks an SM (unpacking alone 230,
@@ -21,7 +21,6 @@ int gemm_q4_long(const Q4Args& G, int bn, cudaStream_t stream);     // gemm_q4_l
 
 namespace {
 
-constexpr int QG_THREADS = 320;                          // warp 0: copies, 1: tensor memory + products, 2..5: unpacking, 6..9: sums
 constexpr int QG_STAGES_MAX = 12;
 
 template <int BN> struct QgShape {
@@ -29,6 +28,8 @@ template <int BN> struct QgShape {
     static constexpr int NA = BN <= 64 ? 2 : 4;                           // unpacked blocks in turn, 64 columns each
     static constexpr int ND = BN <= 32 ? 4 : 2;                           // groups' sums in turn
     static constexpr int PER_SM = BN <= 64 ? 2 : 1;
+    static constexpr int PARTS = BN == 128 ? 2 : 1, CW = BN / PARTS;      // of the tokens, a summing warp one (two at 64: 1 to 8 % slower, at 128: 10 % faster)
+    static constexpr int THREADS = 32 * (6 + 4 * PARTS);                  // warp 0: copies, 1: tensor memory + products, 2..5: unpacking, 6..: sums
     static constexpr uint32_t COLS = BN <= 64 ? 256 : 512;
     static constexpr int D_COL = NA * 64;
     static constexpr int SMEM_MOST = PER_SM == 2 ? 112 * 1024 : 226 * 1024;
@@ -36,10 +37,10 @@ template <int BN> struct QgShape {
 };
 
 template <int BN, int GROUP, bool ZEROS>
-__global__ void __launch_bounds__(QG_THREADS, QgShape<BN>::PER_SM)
+__global__ void __launch_bounds__(QgShape<BN>::THREADS, QgShape<BN>::PER_SM)
 gemm_q4_kernel(const __grid_constant__ CUtensorMap map_x, const Q4Args G) {
     using Sh = QgShape<BN>;
-    constexpr int NA = Sh::NA, ND = Sh::ND, GROUPS = Q4_K / GROUP;
+    constexpr int NA = Sh::NA, ND = Sh::ND, GROUPS = Q4_K / GROUP, CW = Sh::CW, SUMS = 4 * Sh::PARTS;
     extern __shared__ unsigned char smem_raw[];
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_word;
@@ -47,11 +48,11 @@ gemm_q4_kernel(const __grid_constant__ CUtensorMap map_x, const Q4Args G) {
     const uint32_t ring = (smem_addr(smem_raw) + 1023) & ~1023u;             // a stage: tokens, then packed weights
     const int S = G.stages;
     const uint32_t full = ring + S * G.stage_bytes;
-    const uint32_t empty = full + 8 * S;                 // 4 unpacking warps, 4 summing warps
+    const uint32_t empty = full + 8 * S;                 // 4 unpacking warps, all summing warps
     const uint32_t a_full = empty + 8 * S;               // [NA] 4 unpacking warps
-    const uint32_t a_empty = a_full + 8 * NA;            // [NA] 4 summing warps: its products are done
+    const uint32_t a_empty = a_full + 8 * NA;            // [NA] all summing warps: its products are done
     const uint32_t d_full = a_empty + 8 * NA;            // [ND] the products
-    const uint32_t d_empty = d_full + 8 * ND;            // [ND] 4 summing warps
+    const uint32_t d_empty = d_full + 8 * ND;            // [ND] all summing warps
     float* red = reinterpret_cast<float*>(smem_raw + (ring - smem_addr(smem_raw)));       // the sums, [token][row], in the ring once it is idle
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -61,9 +62,9 @@ gemm_q4_kernel(const __grid_constant__ CUtensorMap map_x, const Q4Args G) {
     auto groups_of = [&](int i) { return GROUPS == 1 || i + 1 < n_k ? GROUPS : min(GROUPS, last); };
 
     if (threadIdx.x == 0) {
-        for (int s = 0; s < S; ++s) { q4_init(full + 8 * s, 1); q4_init(empty + 8 * s, 8); }
-        for (int b = 0; b < NA; ++b) { q4_init(a_full + 8 * b, 4); q4_init(a_empty + 8 * b, 4); }
-        for (int b = 0; b < ND; ++b) { q4_init(d_full + 8 * b, 1); q4_init(d_empty + 8 * b, 4); }
+        for (int s = 0; s < S; ++s) { q4_init(full + 8 * s, 1); q4_init(empty + 8 * s, 4 + SUMS); }
+        for (int b = 0; b < NA; ++b) { q4_init(a_full + 8 * b, 4); q4_init(a_empty + 8 * b, SUMS); }
+        for (int b = 0; b < ND; ++b) { q4_init(d_full + 8 * b, 1); q4_init(d_empty + 8 * b, SUMS); }
         abort_word = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -77,7 +78,7 @@ gemm_q4_kernel(const __grid_constant__ CUtensorMap map_x, const Q4Args G) {
     const uint32_t tmem = tmem_slot;
     const int quarter = warp & 3;                        // the lanes of tensor memory a warp reaches: 32 * (warp % 4)
     const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
-    float acc[BN];                                       // of the summing warps: a row's outputs
+    float acc[CW];                                       // of the summing warps: a row's outputs
 
     if (warp == 0) {
         if (lane == 0) {
@@ -182,9 +183,9 @@ gemm_q4_kernel(const __grid_constant__ CUtensorMap map_x, const Q4Args G) {
         }
     } else {
         // ---------------------------------------------------------------- sums
-        const int row = quarter * 32 + lane;
+        const int row = quarter * 32 + lane, part = (warp - 6) >> 2;
 #pragma unroll
-        for (int c = 0; c < BN; ++c) acc[c] = 0.f;
+        for (int c = 0; c < CW; ++c) acc[c] = 0.f;
         grid_dependency_wait();                          // the output may still be read by the kernel in front
         bool ok = true;
         for (int i = 0, s = 0, d = 0; i < n_k && ok; ++i) {
@@ -201,15 +202,15 @@ gemm_q4_kernel(const __grid_constant__ CUtensorMap map_x, const Q4Args G) {
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 if (g == gs - 1 && lane == 0) q4_arrive(a_empty + 8 * (i % NA));
                 const float sc = q4_lds_scale(scales, g * Q4_ROWS + row, G.form.scale_f32);
-                const uint32_t at = lanes + Sh::D_COL + c * BN;
+                const uint32_t at = lanes + Sh::D_COL + c * BN + part * CW;
                 constexpr int AT_ONCE = 16;
 #pragma unroll
-                for (int c0 = 0; c0 < BN; c0 += AT_ONCE) {
+                for (int c0 = 0; c0 < CW; c0 += AT_ONCE) {
                     float r[AT_ONCE / 16][16];
 #pragma unroll
                     for (int j = 0; j < AT_ONCE / 16; ++j) q4_ld16(at + c0 + 16 * j, r[j]);
                     tmem_ld_wait();
-                    if (c0 + AT_ONCE >= BN) {            // the last of them are in registers
+                    if (c0 + AT_ONCE >= CW) {            // the last of them are in registers
                         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                         __syncwarp();
                         if (lane == 0) {
@@ -222,22 +223,22 @@ gemm_q4_kernel(const __grid_constant__ CUtensorMap map_x, const Q4Args G) {
                 }
             }
         }
-        asm volatile("bar.sync 1, 128;" ::: "memory");   // the other summing warps have read their scales out of the ring
+        asm volatile("bar.sync 1, %0;" ::"n"(32 * SUMS) : "memory");   // the other summing warps have read their scales out of the ring
         if (ok && nz == 1 && !G.gate) {
             const int n = tile * Q4_ROWS + row;
             if (n < G.N) {
 #pragma unroll
-                for (int c = 0; c < BN; ++c)
-                    if (t0 + c < G.T) q4_store(G, (size_t)(t0 + c) * G.ldo + n, acc[c]);
+                for (int c = 0; c < CW; ++c)
+                    if (t0 + part * CW + c < G.T) q4_store(G, (size_t)(t0 + part * CW + c) * G.ldo + n, acc[c]);
             }
         } else if (ok) {                                 // the sums to shared memory, [token][row]: the ring is idle, every copy has been waited for
 #pragma unroll
-            for (int c = 0; c < BN; ++c) red[c * Q4_ROWS + row] = acc[c];
+            for (int c = 0; c < CW; ++c) red[(part * CW + c) * Q4_ROWS + row] = acc[c];
         }
     }
     if (nz > 1 || G.gate) {
         if (nz > 1) pair_cluster_sync(); else __syncthreads();
-        if (warp >= 2 && !*abort_flag) q4_finish<1, BN>(G, red, tile, t0, nz, blockIdx.z, (int)threadIdx.x - 64, QG_THREADS - 64);
+        if (warp >= 2 && !*abort_flag) q4_finish<1, BN>(G, red, tile, t0, nz, blockIdx.z, (int)threadIdx.x - 64, Sh::THREADS - 64);
         if (nz > 1) pair_cluster_sync();                 // nobody leaves while its shared memory is read
     }
     // -------------------------------------------------------------------- teardown
@@ -268,7 +269,7 @@ int qg_launch(const CUtensorMap& map, Q4Args G, int tiles, int splits, cudaStrea
     if (ring < (size_t)BN * Q4_ROWS * 4) { G.stages = (int)(((size_t)BN * Q4_ROWS * 4 + G.stage_bytes - 1) / G.stage_bytes); ring = (size_t)G.stages * G.stage_bytes; }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(tiles, (G.T + BN - 1) / BN, splits);
-    cfg.blockDim = dim3(QG_THREADS);
+    cfg.blockDim = dim3(Sh::THREADS);
     cfg.dynamicSmemBytes = ring + 1024 + BARS;
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
@@ -302,8 +303,8 @@ struct QgPlan { int bn, long_, splits, first; double us; };      // tokens of a 
 // Ranges of K in clusters, for one launch over `tiles` of `bn` tokens.  An SM that has two thread blocks takes 1.4 times as long for a block of k of
 // each; of 148 SMs about 133 get a block in clusters of two or three, 118 in clusters of four and 98 in larger ones (of two a SM 266, of seven and
 // more 252), and clusters that find no room begin when others have ended.  Measured at 1, 2 .. 8 ranges, us:  45 tokens, 40 tiles x 108 blocks of k
-// 57 33 24 25 22 19 28 26;  64, 28 x 148: 77 44 31 25 27 24 23 20;  64, 216 x 40: 37 38 47 48 50 56;  128, 28 x 148: 76 48 35 28 46 40 .. 34;
-// 90, 16 x 32: 21 18 14 11.4 10.6 10 .. 16.
+// 57 33 24 25 22 19 28 26;  64, 28 x 148: 77 44 31 25 27 24 23 20;  64, 216 x 40: 37 38 47 48 50 56;  128, 28 x 148: 70 44 32 25 41 36;
+// 128, 74 x 28: 18 19 28 33;  90, 16 x 32: 19 15 12 9.8 9.2 8.7.
 QgPlan qg_ranges(long long tiles, int blocks, int bn) {
     const int sms = tl_num_sms(), two = bn <= 64;
     QgPlan p{bn, 0, 1, 0, 0};
@@ -313,7 +314,7 @@ QgPlan qg_ranges(long long tiles, int blocks, int bn) {
         const long long total = tiles * s, alone = s == 1 ? sms : s <= 3 ? sms * 9 / 10 : s == 4 ? sms * 4 / 5 : sms * 2 / 3;
         const long long both = s == 1 ? 2 * sms : s <= 6 ? sms * 9 / 5 : sms * 17 / 10;
         const double turns = total <= alone ? 1 : two ? 1.4 * ((total + both - 1) / both) : (total + alone - 1) / alone;
-        const double us = two ? turns * (per + 4) * (bn == 32 ? 0.5 : 0.6) + 2 : turns * (per * 0.55 + 10);
+        const double us = two ? turns * (per + 4) * (bn == 32 ? 0.5 : 0.6) + 2 : turns * (per * 0.44 + (s == 1 ? 5.5 : 9));
         if (s == 1 || us < p.us) { p.splits = s; p.us = us; }
     }
     return p;
@@ -321,7 +322,7 @@ QgPlan qg_ranges(long long tiles, int blocks, int bn) {
 
 // One launch.  The blocks of gemm_q4_long.cu, one a SM, take a block of k through in 410, 420, 450 and 520 ns at 32, 64, 96 and 128 tokens: of its
 // tiles, the one with which they are done first.  Up to 64 tokens, and where there are so few tiles that many SMs would have none, ranges of K
-// in clusters are faster.  Measured, us, here / there:  128 tokens, 28 tiles x 148 blocks of k 28 / 65;  74 x 28 22 / 15.5;  256 tokens, 28 x 148 49 / 68.
+// in clusters are faster.  Measured, us, here / there:  128 tokens, 28 tiles x 148 blocks of k 25 / 65;  74 x 28 18 / 15.6;  256 tokens, 28 x 148 45 / 68.
 QgPlan qg_one(int T, int m_tiles, int blocks) {
     const int here = T <= 32 ? 32 : T <= 64 ? 64 : 128, sms = tl_num_sms();
     QgPlan p = qg_ranges((long long)m_tiles * ((T + here - 1) / here), blocks, here);

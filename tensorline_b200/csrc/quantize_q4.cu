@@ -8,14 +8,14 @@
 // is no number or infinite has a scale that is no number, so that whoever reads it sees it.
 //
 // Both kernels move a matrix once: a block of threads takes 128 rows and 128 k, 16 lanes a row, eight k a lane (one word of codes).  Reading back is
-// bound by that; making codes by its instructions, about 24 a value, although quotients are decided exactly without 64-bit arithmetic
-// (q4_round).  Measured, 37,888 x 3,584 in groups of 128: codes from bfloat16 123 us (floor 52), from float 145 (94); values in bfloat16 54 us
+// bound by that; making codes by its instructions, about 20 a value, although quotients are decided exactly without 64-bit arithmetic
+// (q4_round).  Measured, 37,888 x 3,584 in groups of 128: codes from bfloat16 113 us (floor 52), from float 108 (94); values in bfloat16 54 us
 // (52), in float 98 (94).
 #include "q4.cuh"
 
 namespace {
 
-constexpr int QQ_THREADS = 256;
+constexpr int QQ_THREADS = 256;                          // of a block that reads back
 
 // The nearest whole number to w / s, ties to even, as the last bits of a float: added to 1.5 2^23, a value is rounded to a whole number.  For
 // 2^-100 <= s and |w| <= 16 s.  The quotient by the reciprocal is off by less than 2^-18, so this is the nearest number to w / s or, around
@@ -25,6 +25,19 @@ __device__ __forceinline__ float q4_round(float w, float s, float inv, float& fa
     const float t = __fmaf_rn(w, inv, Q4_MAGIC);
     far = fmaxf(far, fabsf(__fmaf_rn(-s, t - Q4_MAGIC, w)));
     return t;
+}
+// two at a time, in this architecture's pairs of float operations
+__device__ __forceinline__ void q4_round2(float w0, float w1, float s, float inv, float& t0, float& t1, float& far) {
+    float l0, l1;
+    asm("{\n\t.reg .b64 w, i, m, t, n, c, l;\n\t"
+        "mov.b64 w, {%4, %5};\n\tmov.b64 i, {%6, %6};\n\tmov.b64 m, {%8, %8};\n\tmov.b64 n, {%9, %9};\n\t"
+        "fma.rn.f32x2 t, w, i, m;\n\t"
+        "add.rn.f32x2 c, t, n;\n\t"
+        "mov.b64 i, {%7, %7};\n\t"
+        "fma.rn.f32x2 l, i, c, w;\n\t"
+        "mov.b64 {%0, %1}, t;\n\tmov.b64 {%2, %3}, l;\n\t}"
+        : "=f"(t0), "=f"(t1), "=f"(l0), "=f"(l1) : "f"(w0), "f"(w1), "f"(inv), "f"(-s), "f"(Q4_MAGIC), "f"(-Q4_MAGIC));
+    far = fmaxf(far, fmaxf(fabsf(l0), fabsf(l1)));
 }
 __device__ __forceinline__ float q4_mend(float w, float s, float t) {
     const float left = __fmaf_rn(-s, t - Q4_MAGIC, w), far = fabsf(left), half = 0.5f * s;
@@ -67,11 +80,13 @@ __device__ __forceinline__ void q4_widen(const uint4 (&q)[2], float (&v)[8]) {
     }
 }
 
-// A thread's eight rows are asked for at once (one behind the other they were 1.3 times the time).
+// A thread's rows are asked for at once (one behind the other they were 1.3 times the time): eight of bfloat16, four of float, whose
+// registers leave room for fewer threads (four rows of bfloat16: 118 us instead of 113, eight of float: 140 instead of 108).
+template <typename T> constexpr int QQ_MAKE = sizeof(T) == 2 ? 256 : 512;
 template <typename T, bool ZEROS>
-__global__ void __launch_bounds__(QQ_THREADS)
+__global__ void __launch_bounds__(QQ_MAKE<T>)
 quantize_q4_kernel(const T* __restrict__ w, unsigned char* __restrict__ out, int N, int K, int blocks, const Q4Form form) {
-    constexpr int PIECES = sizeof(T) / 2, ROUNDS = Q4_ROWS / (QQ_THREADS / 16);
+    constexpr int PIECES = sizeof(T) / 2, THREADS = QQ_MAKE<T>, ROUNDS = Q4_ROWS / (THREADS / 16);
     __shared__ __align__(16) unsigned char tile[Q4_CODES + 4 * Q4_ROWS * 4 + 4 * Q4_ROWS];
     grid_dependency_wait();
     const int kb = blockIdx.x, row0 = blockIdx.y * Q4_ROWS;
@@ -80,7 +95,7 @@ quantize_q4_kernel(const T* __restrict__ w, unsigned char* __restrict__ out, int
     uint4 raw[ROUNDS][PIECES];
 #pragma unroll
     for (int i = 0; i < ROUNDS; ++i) {
-        const int r = row0 + r0 + i * (QQ_THREADS / 16);
+        const int r = row0 + r0 + i * (THREADS / 16);
 #pragma unroll
         for (int j = 0; j < PIECES; ++j) {
             raw[i][j] = make_uint4(0u, 0u, 0u, 0u);
@@ -89,7 +104,7 @@ quantize_q4_kernel(const T* __restrict__ w, unsigned char* __restrict__ out, int
     }
 #pragma unroll
     for (int i = 0; i < ROUNDS; ++i) {
-        const int r = r0 + i * (QQ_THREADS / 16);
+        const int r = r0 + i * (THREADS / 16);
         float v[8];
         q4_widen(raw[i], v);
         float lo = 0.f, hi = 0.f;                        // without zeros `hi` is the largest magnitude; no number, or infinite, if a value is
@@ -115,7 +130,7 @@ quantize_q4_kernel(const T* __restrict__ w, unsigned char* __restrict__ out, int
                 zero = __float_as_int(q4_mend(-lo, s, q4_round(-lo, s, inv, z))) - __float_as_int(Q4_MAGIC);      // 0 .. 15: the scale is within 2^-8
             }
 #pragma unroll
-            for (int j = 0; j < 8; ++j) t[j] = q4_round(v[j], s, inv, far);
+            for (int j = 0; j < 8; j += 2) q4_round2(v[j], v[j + 1], s, inv, t[j], t[j + 1], far);
             if (far >= 0.5f * s)
 #pragma unroll
                 for (int j = 0; j < 8; ++j) t[j] = q4_mend(v[j], s, t[j]);
@@ -142,7 +157,7 @@ quantize_q4_kernel(const T* __restrict__ w, unsigned char* __restrict__ out, int
     }
     __syncthreads();
     uint4* dst = reinterpret_cast<uint4*>(out + ((size_t)blockIdx.y * blocks + kb) * form.bytes);
-    for (int i = threadIdx.x; i < form.bytes / 16; i += QQ_THREADS) dst[i] = reinterpret_cast<const uint4*>(tile)[i];
+    for (int i = threadIdx.x; i < form.bytes / 16; i += THREADS) dst[i] = reinterpret_cast<const uint4*>(tile)[i];
 }
 
 __device__ __forceinline__ void q4_store8(float* dst, const float (&v)[8]) {      // (two stores of 16 bytes, 32 apart: 142 us instead of 98 for 136 million)
@@ -203,7 +218,7 @@ TL_EXPORT int tl_quantize_q4(const void* w, int w_f32, void* out, int N, int K, 
     Q4Form form;
     dim3 grid;
     if (N < 1 || K < 1 || (K & 7) || form_bits < 0 || form_bits >> 10 || !q4_form(&form, form_bits & 255, form_bits >> 8 & 1, form_bits >> 9 & 1) || !q4_grid(&grid, N, K) || ((uintptr_t)w & 15) || ((uintptr_t)out & 15)) return 1;
-    auto run = [&](auto kernel, auto matrix) { return launch_after_wait(kernel, grid, dim3(QQ_THREADS), 0, stream, matrix, (unsigned char*)out, N, K, (int)grid.x, form); };
+    auto run = [&](auto kernel, auto matrix) { return launch_after_wait(kernel, grid, dim3(w_f32 ? QQ_MAKE<float> : QQ_MAKE<bf16>), 0, stream, matrix, (unsigned char*)out, N, K, (int)grid.x, form); };
     if (w_f32) return form.zeros ? run(quantize_q4_kernel<float, true>, (const float*)w) : run(quantize_q4_kernel<float, false>, (const float*)w);
     return form.zeros ? run(quantize_q4_kernel<bf16, true>, (const bf16*)w) : run(quantize_q4_kernel<bf16, false>, (const bf16*)w);
 }

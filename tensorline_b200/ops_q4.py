@@ -207,6 +207,17 @@ def _gate(gated):
     raise KernelError(f"a gated epilogue applies 'silu', 'gelu_tanh' or ('swish_clamped', limit, alpha), not {gated!r}")
 
 
+def _meet(a: int, a_step: int, a_bytes: int, b: int, b_step: int, b_bytes: int, rows: int) -> bool:
+    """Whether two matrices of `rows` rows share memory (addresses, bytes from row to row and of a row); said of some that only interlace too,
+    but not of columns of one matrix."""
+    if rows == 0 or a + (rows - 1) * a_step + a_bytes <= b or b + (rows - 1) * b_step + b_bytes <= a:
+        return False
+    if rows > 1 and a_step == b_step:
+        ahead = (b - a) % a_step
+        return ahead < a_bytes or ahead + b_bytes > a_step
+    return True
+
+
 # A call takes the host 7 us and the smallest products 5 us, so what is asked of a tensor is asked once, and nothing is built that the call does
 # not need (10.5 us with properties of the device and an argument for each of the weights' properties).
 def gemm_q4(x: torch.Tensor, w: Q4Weight, out_dtype: torch.dtype = torch.bfloat16, *, gated=False, out: torch.Tensor | None = None) -> torch.Tensor:
@@ -214,7 +225,7 @@ def gemm_q4(x: torch.Tensor, w: Q4Weight, out_dtype: torch.dtype = torch.bfloat1
     Rows of x may lie apart (a multiple of 8 values); T may be 0.
     `gated` ("silu", "gelu_tanh" or ("swish_clamped", limit, alpha)): w holds gate and up rows alternating in blocks of 64 (N a multiple of
     128), the result is act(gate) * up, [T, N / 2], from the float32 sums.  `out`: a tensor to write, of the result's shape and type, with rows
-    that may lie apart."""
+    that may lie apart, that shares no memory with x."""
     n, k, data = w.n, w.k, w.data
     form, limit, alpha = w.form, 0.0, 1.0
     if gated:
@@ -251,6 +262,8 @@ def gemm_q4(x: torch.Tensor, w: Q4Weight, out_dtype: torch.dtype = torch.bfloat1
         if out.shape != (T, cols) or out.dtype is not out_dtype or (cols > 1 and out.stride(1) != 1) or ldo < cols:
             raise KernelError(f"gemm_q4: out is {out_dtype} [{T}, {cols}] with unit inner stride")
         _device(x, out)
+        if _meet(ptr, ldx * 2, k * 2, out.data_ptr(), ldo * out_dtype.itemsize, cols * out_dtype.itemsize, T):
+            raise KernelError("gemm_q4: out shares memory with x")
     if T == 0:
         return out
     if index != torch._C._cuda_getDevice():

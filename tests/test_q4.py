@@ -72,6 +72,18 @@ def test_sizes_that_the_entries_have_no_room_for():
         ops_q4.Q4Weight(torch.empty(2 ** 25, 1, 8448, dtype=torch.uint8, device="meta"), 2 ** 32, 128)
 
 
+def test_matrices_that_share_memory():
+    n = 10
+    for a, a_step, a_bytes, b, b_step, b_bytes, rows in [(1000, 200, 64, 1000 + at, step, wide, n) for at in range(-2300, 2300, 20) for step in (80, 200, 320) for wide in (20, 80)]:
+        bytes_of = lambda start, by, wide: {start + r * by + c for r in range(rows) for c in range(wide)}      # noqa: E731
+        shared = bool(bytes_of(a, a_step, a_bytes) & bytes_of(b, b_step, b_bytes))
+        said = ops_q4._meet(a, a_step, a_bytes, b, b_step, b_bytes, rows)
+        assert said >= shared                            # never missed
+        if a_step == b_step:
+            assert said == shared
+    assert not ops_q4._meet(0, 64, 64, 0, 64, 64, 0) and ops_q4._meet(0, 0, 64, 32, 0, 64, 1) and not ops_q4._meet(0, 0, 64, 64, 0, 64, 1)
+
+
 def test_entries_are_declared_as_they_are_called():
     import ctypes
     import os

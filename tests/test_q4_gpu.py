@@ -300,6 +300,19 @@ def test_refusals(q4):
     assert torch.equal(q4.gemm_q4(x[2:3].expand(1, 64), w), q4.gemm_q4(x, w)[2:3])
 
 
+@pytest.mark.parametrize("T", [1, 40, 200])
+def test_outputs_beside_tokens_not_in_them(q4, T):
+    from tensorline_b200.ops import KernelError
+    w, _ = whole(q4, 128, 128, 64, False, BF)
+    room = torch.zeros(T + 1, 256, dtype=BF, device="cuda")
+    room[:T, :128] = whole_x(T, 128)
+    x, want = room[:T, :128], q4.gemm_q4(whole_x(T, 128), w)
+    for out in (x, room[:T, 64:192], room[1:, :128] if T > 1 else x):
+        with pytest.raises(KernelError, match="shares memory"):
+            q4.gemm_q4(x, w, out=out)
+    assert torch.equal(q4.gemm_q4(x, w, out=room[:T, 128:]), want) and torch.equal(room[:T, :128], whole_x(T, 128))
+
+
 # ------------------------------------------------------------------ streams, graphs, one call behind another
 def test_made_and_used_without_a_wait(q4):
     """Weights that the kernel in front is still writing: a product that was not promised anything waits for them."""

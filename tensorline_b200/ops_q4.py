@@ -137,8 +137,10 @@ def quantize(w: torch.Tensor, group: int = 128, zeros: bool = False, scale_dtype
     if (other := _on(index)) is not None:
         with other:
             return quantize(w, group, zeros, scale_dtype)
-    q = Q4Weight(torch.empty((-(-n // ROWS), -(-k // K_BLOCK), size), dtype=torch.uint8, device=w.device), n, k, group, zeros, scale_dtype)
-    _check(lib().tl_quantize_q4(w.data_ptr(), int(w.dtype is torch.float32), q.data.data_ptr(), n, k, q.form, _stream()), "quantize_q4")
+    blocks = -(-k // K_BLOCK)
+    data = torch.empty_strided((-(-n // ROWS), blocks, size), (blocks * size, size, 1), dtype=torch.uint8, device=w.device)
+    q = Q4Weight(data, n, k, group, zeros, scale_dtype)
+    _check(lib().tl_quantize_q4(w.data_ptr(), int(w.dtype is torch.float32), data.data_ptr(), n, k, q.form, _stream()), "quantize_q4")
     return q
 
 
@@ -151,7 +153,7 @@ def dequantize(w: Q4Weight, dtype: torch.dtype = torch.float32) -> torch.Tensor:
     if (other := _on(_device(w.data))) is not None:
         with other:
             return dequantize(w, dtype)
-    out = torch.empty(w.shape, dtype=dtype, device=w.data.device)
+    out = torch.empty_strided((w.n, w.k), (w.k, 1), dtype=dtype, device=w.data.device)      # (0.8 us less of the host's time than `empty`)
     _check(lib().tl_dequantize_q4(w.data.data_ptr(), out.data_ptr(), int(dtype is torch.float32), w.n, w.k, w.form, _stream()), "dequantize_q4")
     return out
 

@@ -8,8 +8,8 @@
 // is no number or infinite has a scale that is no number, so that whoever reads it sees it.
 //
 // Both kernels move a matrix once: a block of threads takes 128 rows and 128 k, 16 lanes a row, eight k a lane (one word of codes).  Reading back is
-// bound by that; making codes by its instructions, about 20 a value, although quotients are decided exactly without 64-bit arithmetic
-// (q4_round).  Measured, 37,888 x 3,584 in groups of 128: codes from bfloat16 113 us (floor 52), from float 108 (94); values in bfloat16 54 us
+// bound by that; making codes from bfloat16 by its instructions, 18 a value, although quotients are decided exactly without 64-bit arithmetic
+// (q4_round).  Measured, 37,888 x 3,584 in groups of 128: codes from bfloat16 86 us (floor 52), from float 95 (94); values in bfloat16 54 us
 // (52), in float 98 (94).
 #include "q4.cuh"
 
@@ -81,9 +81,10 @@ __device__ __forceinline__ void q4_widen(const uint4 (&q)[2], float (&v)[8]) {
 }
 
 // A thread's rows are asked for at once (one behind the other they were 1.3 times the time): eight of bfloat16, four of float, whose
-// registers leave room for fewer threads (four rows of bfloat16: 118 us instead of 113, eight of float: 140 instead of 108).
+// registers leave room for fewer threads (four rows of bfloat16: 4 % slower, eight of float: 30 %).  The group is the kernel's own, so that the
+// lanes' exchange is a straight run of instructions (a loop over them: 113 us instead of 86).
 template <typename T> constexpr int QQ_MAKE = sizeof(T) == 2 ? 256 : 512;
-template <typename T, bool ZEROS>
+template <typename T, bool ZEROS, int GROUP>
 __global__ void __launch_bounds__(QQ_MAKE<T>)
 quantize_q4_kernel(const T* __restrict__ w, unsigned char* __restrict__ out, int N, int K, int blocks, const Q4Form form) {
     constexpr int PIECES = sizeof(T) / 2, THREADS = QQ_MAKE<T>, ROUNDS = Q4_ROWS / (THREADS / 16);
@@ -91,7 +92,8 @@ quantize_q4_kernel(const T* __restrict__ w, unsigned char* __restrict__ out, int
     grid_dependency_wait();
     const int kb = blockIdx.x, row0 = blockIdx.y * Q4_ROWS;
     const int lane = threadIdx.x & 31, m = lane & 15, k = kb * Q4_K + 8 * m, r0 = (threadIdx.x >> 5) * 2 + (lane >> 4);
-    const int lanes = form.group / 8, scales_at = Q4_CODES, zeros_at = scales_at + form.groups * Q4_ROWS * (form.scale_f32 ? 4 : 2);
+    constexpr int lanes = GROUP / 8, scales_at = Q4_CODES;
+    const int zeros_at = scales_at + Q4_K / GROUP * Q4_ROWS * (form.scale_f32 ? 4 : 2);
     uint4 raw[ROUNDS][PIECES];
 #pragma unroll
     for (int i = 0; i < ROUNDS; ++i) {
@@ -113,6 +115,7 @@ quantize_q4_kernel(const T* __restrict__ w, unsigned char* __restrict__ out, int
             hi = q4_max_nan(hi, ZEROS ? v[j] : fabsf(v[j]));
             if (ZEROS) lo = q4_min_nan(lo, v[j]);
         }
+#pragma unroll
         for (int o = 1; o < lanes; o <<= 1) {
             hi = q4_max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
             if (ZEROS) lo = q4_min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, o));
@@ -219,8 +222,14 @@ TL_EXPORT int tl_quantize_q4(const void* w, int w_f32, void* out, int N, int K, 
     dim3 grid;
     if (N < 1 || K < 1 || (K & 7) || form_bits < 0 || form_bits >> 10 || !q4_form(&form, form_bits & 255, form_bits >> 8 & 1, form_bits >> 9 & 1) || !q4_grid(&grid, N, K) || ((uintptr_t)w & 15) || ((uintptr_t)out & 15)) return 1;
     auto run = [&](auto kernel, auto matrix) { return launch_after_wait(kernel, grid, dim3(w_f32 ? QQ_MAKE<float> : QQ_MAKE<bf16>), 0, stream, matrix, (unsigned char*)out, N, K, (int)grid.x, form); };
-    if (w_f32) return form.zeros ? run(quantize_q4_kernel<float, true>, (const float*)w) : run(quantize_q4_kernel<float, false>, (const float*)w);
-    return form.zeros ? run(quantize_q4_kernel<bf16, true>, (const bf16*)w) : run(quantize_q4_kernel<bf16, false>, (const bf16*)w);
+    auto typed = [&](auto matrix, auto zeros) {
+        using T = std::remove_const_t<std::remove_pointer_t<decltype(matrix)>>;
+        constexpr bool Z = decltype(zeros)::value;
+        return form.group == 128 ? run(quantize_q4_kernel<T, Z, 128>, matrix) : form.group == 64 ? run(quantize_q4_kernel<T, Z, 64>, matrix)
+                                                                              : run(quantize_q4_kernel<T, Z, 32>, matrix);
+    };
+    if (w_f32) return form.zeros ? typed((const float*)w, std::true_type()) : typed((const float*)w, std::false_type());
+    return form.zeros ? typed((const bf16*)w, std::true_type()) : typed((const bf16*)w, std::false_type());
 }
 
 // The values that weights of 4 bits stand for, [N, K] bfloat16 or float (on a 32-byte boundary).

@@ -8,7 +8,7 @@
 // is no number or infinite has a scale that is no number, so that whoever reads it sees it.
 //
 // Both kernels move a matrix once: a block of threads takes 128 rows and 128 k, 16 lanes a row, eight k a lane (one word of codes).  Reading back is
-// bound by that; making codes from bfloat16 by its instructions, 18 a value, although quotients are decided exactly without 64-bit arithmetic
+// bound by that; making codes from bfloat16 by its instructions, 17 a value, although quotients are decided exactly without 64-bit arithmetic
 // (q4_round).  Measured, 37,888 x 3,584 in groups of 128: codes from bfloat16 86 us (floor 52), from float 95 (94); values in bfloat16 54 us
 // (52), in float 98 (94).
 #include "q4.cuh"

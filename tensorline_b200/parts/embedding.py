@@ -17,13 +17,14 @@ class Embedding(Part):
         `copies`: the stream starts as that many equal copies side by side, [T, copies * dim]."""
         super().__init__(rt)
         self.vocab, self.dim, self.tensor, self.scale, self.copies = vocab, dim, tensor, float(scale), int(copies)
-        self.weight = None
+        self.weight = self.stored_as = None              # the table as it is read; the name it was bound from
 
     def expected_tensors(self, prefix):
         return {tensor_name(prefix, self.tensor): TensorSpec((self.vocab, self.dim))}
 
     def bind(self, weights, prefix):
-        self.weight = self._compute_copy(weights[tensor_name(prefix, self.tensor)])
+        self.stored_as = tensor_name(prefix, self.tensor)
+        self.weight = self._compute_copy(weights[self.stored_as])
 
     def forward(self, ids):
         """The residual stream starts here, in float32."""
@@ -94,7 +95,9 @@ class LMHead(Part):
 
     def bind(self, weights, prefix, embedding: Embedding | None = None):
         if self.tied:
-            self.weight = self._matrix(embedding.weight) if self.rt.quantize_head else embedding.weight
+            self.weight = embedding.weight
+            if self.rt.quantize_head:                    # as every matrix from the stored values, which the embedding may have rounded
+                self.weight = self._matrix(weights.get(getattr(embedding, "stored_as", None), embedding.weight))
         else:
             stored = weights[tensor_name(prefix, self.tensor)]
             self.weight = self._matrix(stored) if self.rt.quantize_head else self._compute_copy(stored)

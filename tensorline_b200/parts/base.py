@@ -97,7 +97,7 @@ class Part:
         if self.rt.weight_bits != 4 or t.shape[1] % 8:
             return self._compute_copy(t)
         from .. import ops_q4
-        t = t.contiguous()
+        t = (t if t.dtype in (torch.bfloat16, torch.float32) else t.float()).contiguous()       # (as a folder's loader has it)
         q = ops_q4.quantize(t.clone() if t.data_ptr() % 16 else t, self.rt.weight_group, self.rt.weight_zeros)
         if self.rt.exact:
             return ops_q4.dequantize(q)

@@ -29,3 +29,15 @@ def test_a_tied_head_is_made_from_the_table_as_it_is_stored(quantized, act, stor
     head.bind(weights, "head", embedding)
     assert len(quantized) == 1 and quantized[0].dtype == stored and torch.equal(quantized[0], table)
     assert embedding.weight.dtype == (torch.bfloat16 if act == torch.bfloat16 else stored)      # the table itself stays as it is
+
+
+@pytest.mark.parametrize("stored", [torch.float16, torch.float64])
+def test_matrices_of_other_types_by_way_of_float32(quantized, stored):
+    from tensorline_b200.parts import FEED_FORWARDS
+    rt = Runtime(torch.device("cpu"), torch.bfloat16, weight_bits=4)
+    part = FEED_FORWARDS.build(PartSpec("plain_mlp", dict(hidden=16, intermediate=24)), rt)
+    g = torch.Generator().manual_seed(2)
+    weights = {n: torch.randn(s.shape, generator=g).to(stored) for n, s in part.expected_tensors("l").items()}
+    part.bind(weights, "l")
+    for seen, name in zip(quantized, ("l.up_proj.weight", "l.down_proj.weight"), strict=True):
+        assert seen.dtype == torch.float32 and torch.equal(seen, weights[name].float())

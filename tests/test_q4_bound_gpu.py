@@ -22,3 +22,17 @@ def test_a_tied_head_holds_the_same_values_in_both_engines(tmp_path, store):
         head = engine(folder, dtype, weight_bits=4, weight_group=32, weight_zeros=True, quantize_head=True).model.head.weight
         values = ops_q4.dequantize(head) if isinstance(head, ops_q4.Q4Weight) else head
         assert values.dtype == torch.float32 and torch.equal(values.cpu(), want), dtype
+
+
+@pytest.mark.parametrize("stored", [torch.float16, torch.float64])
+def test_matrices_of_other_types(stored):
+    """As a folder's loader has it for what no kernel reads: by way of float32."""
+    from tensorline_b200 import ops_q4
+    from tensorline_b200.parts import FEED_FORWARDS, PartSpec, Runtime
+    g = torch.Generator().manual_seed(3)
+    part = FEED_FORWARDS.build(PartSpec("gated_mlp", dict(hidden=64, intermediate=128)), Runtime(torch.device("cuda", 0), torch.bfloat16, weight_bits=4))
+    weights = {n: torch.randn(s.shape, generator=g).to(stored).cuda() for n, s in part.expected_tensors("l").items()}
+    part.bind(weights, "l")
+    codes, scales, _ = quantized(weights["l.down_proj.weight"].float(), 128, False, torch.bfloat16)
+    want = (scales.double().repeat_interleave(128, dim=1)[:, :128] * (codes - 8).double()).float()
+    assert torch.equal(ops_q4.dequantize(part.w_down).cpu(), want)

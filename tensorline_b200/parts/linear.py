@@ -254,14 +254,19 @@ def resolve(t):
     return t.sum() if isinstance(t, SplitSum) else t
 
 
+def product_q4(x, w: ops_q4.Q4Weight, out_dtype: torch.dtype | None = None, gated=False) -> torch.Tensor:
+    """`ops_q4.gemm_q4` of whatever a norm or a projection returned; rows that its copies cannot take as they lie are copied first."""
+    x = resolve(x)
+    plain = x.stride(1) == 1 and x.data_ptr() % 16 == 0 and (x.shape[0] < 2 or (x.stride(0) % 8 == 0 and x.stride(0) >= x.shape[1]))
+    return ops_q4.gemm_q4(x if plain else x.clone(memory_format=torch.contiguous_format), w, out_dtype or x.dtype, gated=gated)
+
+
 def matmul(x, w: torch.Tensor, out_dtype: torch.dtype | None = None, may_defer: bool = False, to_residual: bool = False):
     """x [T, K] (float32 or bfloat16) times w [N, K]^T -> [T, N].  `may_defer`: the caller hands the
     result to a consumer that takes a `SplitSum`.  `to_residual`: the result is an addend of the residual stream and
     goes to a norm's `add_norm`: a `PendingProduct` may come back instead of a result.  `x` may be a `NormedInput`, `w` a `Q4Weight`."""
     if isinstance(w, ops_q4.Q4Weight):                   # sums are whole and scaled in the product's own kernel: nothing is deferred
-        x = resolve(x)
-        plain = x.stride(1) == 1 and x.stride(0) % 8 == 0 and x.data_ptr() % 16 == 0
-        return ops_q4.gemm_q4(x if plain else x.clone(memory_format=torch.contiguous_format), w, out_dtype or x.dtype)
+        return product_q4(x, w, out_dtype)
     if isinstance(x, NormedInput):
         if x.rows is None and use_tc(x.shape[0], w.shape[0], w.shape[1]) and w.dtype == torch.bfloat16:
             from .. import ops_gemm

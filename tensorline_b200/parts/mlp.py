@@ -15,7 +15,7 @@ import torch
 
 from .. import ops, ops_q4
 from .base import Part, Runtime, TensorSpec, register_feed_forward
-from .linear import NormedInput, matmul, resolve, use_pair_product, use_tc
+from .linear import NormedInput, matmul, product_q4, resolve, use_pair_product, use_tc
 
 GATE_BLOCK = 64
 
@@ -60,7 +60,7 @@ class GatedMLP(Part):
     def forward(self, h, ctx):
         I = self.intermediate
         if self.block and isinstance(self.w_gate_up, ops_q4.Q4Weight):         # 4 bits: both projections, the activation and the product in one kernel
-            return matmul(ops_q4.gemm_q4(resolve(h), self.w_gate_up, gated=self.gate), self.w_down)
+            return matmul(product_q4(h, self.w_gate_up, gated=self.gate), self.w_down)
         if isinstance(h, NormedInput) and h.rows is not None:
             h = h.materialize()
         if self.block and h.dtype == torch.bfloat16 and h.is_contiguous() and use_tc(h.shape[0], 2 * I, self.hidden):

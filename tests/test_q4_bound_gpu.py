@@ -36,3 +36,22 @@ def test_matrices_of_other_types(stored):
     codes, scales, _ = quantized(weights["l.down_proj.weight"].float(), 128, False, torch.bfloat16)
     want = (scales.double().repeat_interleave(128, dim=1)[:, :128] * (codes - 8).double()).float()
     assert torch.equal(ops_q4.dequantize(part.w_down).cpu(), want)
+
+
+@pytest.mark.parametrize("kind", ["gated_mlp", "plain_mlp"])
+@pytest.mark.parametrize("cut", ["rows of a wider matrix", "rows between two 16-byte boundaries", "every other value", "one row for all"])
+def test_a_feed_forward_of_rows_that_lie_apart(kind, cut):
+    """As weights of 16 bits take them."""
+    from tensorline_b200.parts import FEED_FORWARDS, PartSpec, Runtime
+    g = torch.Generator().manual_seed(4)
+    wide = torch.randn(5, 140, generator=g).to(torch.bfloat16).cuda()
+    h = {"rows of a wider matrix": lambda: wide[:, :64], "rows between two 16-byte boundaries": lambda: wide[:, 4:68], "every other value": lambda: wide[:, :128:2],
+         "one row for all": lambda: wide[0, :64].expand(5, 64)}[cut]()
+    assert h.shape == (5, 64) and not h.is_contiguous()
+    activation = "silu" if kind == "gated_mlp" else "gelu_tanh"
+    for bits in (None, 4):
+        part = FEED_FORWARDS.build(PartSpec(kind, dict(hidden=64, intermediate=128, activation=activation)), Runtime(torch.device("cuda", 0), torch.bfloat16, weight_bits=bits))
+        part.bind({n: torch.randn(s.shape, generator=g).to(torch.bfloat16).cuda() for n, s in part.expected_tensors("l").items()}, "l")
+        got = part.forward(h, None)
+        if bits == 4:                                    # (a library's product may add up in another order for them)
+            assert torch.equal(got, part.forward(h.contiguous(), None))

@@ -143,6 +143,11 @@ def weight_options(a) -> dict:
     return dict(weight_bits=4, quantize_head=a.quantize_head) if a.weight_bits else {}
 
 
+def precision(a) -> str:
+    """What a line's metric says of the numbers' form."""
+    return "bf16" + (f", weights{' and output head' if a.quantize_head else ''} of 4 bits" if a.weight_bits else "")
+
+
 def weight_bytes_read_per_step(cfg, layers, options=None):
     """Bytes of weights one decode step reads: every matrix of every layer once, the output head, the
     norms; embedding rows are a few KB and left out.  `options`: of `weight_options`."""
@@ -461,7 +466,7 @@ def run_ours(a):
         print(f"[bench] mix: {m['tok_s']:.0f} generated tok/s, {m['total_tok_s']:.0f} tok/s with prompts, "
               f"{m['steps']} steps, {m['preemptions']} preemptions", file=sys.stderr, flush=True)
         line = {
-            "metric": f"continuous-batching generated tok/s ({model['name']} bf16, {MIX['requests']} requests, prompts "
+            "metric": f"continuous-batching generated tok/s ({model['name']} {precision(a)}, {MIX['requests']} requests, prompts "
                       f"U[{MIX['prompt'][0]}, {MIX['prompt'][1]}], outputs U[{MIX['output'][0]}, {MIX['output'][1]}], "
                       f"{MIX['chunk']}-token chunks)",
             "value": round(m["tok_s"], 1), "unit": "tok/s", "n_gpus": 1, "steps": m["steps"], "warmup": int(a.warm_mix),
@@ -492,12 +497,12 @@ def run_ours(a):
         tl = timeline.Timeline({"product": ops_gemm.lib(), "attn": ops_attention.attn_lib(cfg.head_dim)}, device)
         ms, _, _ = timed_decode(eng, batch, ctx0, max(K, 8), W, V)
         tl.stop()
-        print(f"decode step, batch {batch}, context {ctx0}, {L} layers: {ms:.4f} ms with the stamps")
+        print(f"decode step, {precision(a)}, batch {batch}, context {ctx0}, {L} layers: {ms:.4f} ms with the stamps")
         print(timeline.table(tl.last_step(ms)))
         return 0
     if a.only == "prefill":
         pre_ms = timed_prefill(eng, PREFILL_TOKENS, V, iters=max(1, K), warm=W)
-        print(json.dumps({"impl": "ours", "only": "prefill", "layers": L, "tokens": PREFILL_TOKENS, "ms": round(pre_ms, 3)}))
+        print(json.dumps({"impl": "ours", "only": "prefill", "precision": precision(a), "layers": L, "tokens": PREFILL_TOKENS, "ms": round(pre_ms, 3)}))
         return 0
     # The two timed regions run back to back on a GPU that the power limit slows as it warms (three rounds of e2e and
     # device timing in one process: 2.929 / 2.973 ms, then 2.997 / 3.003, 3.000 / 3.009): whichever comes second reads
@@ -512,7 +517,7 @@ def run_ours(a):
     value = batch * 1000.0 / ms
     print(f"[bench] decode b{batch}: {ms:.3f} ms/step, {value:.0f} tok/s", file=sys.stderr, flush=True)
     if a.only == "decode":                                           # a short run for profilers
-        print(json.dumps({"impl": "ours", "only": "decode", "batch": batch, "layers": L, "ms_per_step": round(ms, 4),
+        print(json.dumps({"impl": "ours", "only": "decode", "precision": precision(a), "batch": batch, "layers": L, "ms_per_step": round(ms, 4),
                           "value": round(value, 1), "gpu_launches": launches * K}))
         return 0
     points = {}
@@ -528,7 +533,7 @@ def run_ours(a):
     step_bytes = weight_bytes_read_per_step(cfg, L, weight_options(a)) + kv_bytes
     achieved = step_bytes / (ms * 1e-3) / 1e9
     line = {
-        "metric": f"decode tok/s at batch {batch} ({model['name']} bf16{', weights of 4 bits' if a.weight_bits else ''}, context {context})", "value": round(value, 1), "unit": "tok/s",
+        "metric": f"decode tok/s at batch {batch} ({model['name']} {precision(a)}, context {context})", "value": round(value, 1), "unit": "tok/s",
         "n_gpus": 1, "steps": K, "warmup": W, "ms_per_step": round(ms, 4), "higher_is_better": True,
         "scaling": "weak", "vs_baseline": None, "dtype": "bf16", "data": "synthetic", "impl": "ours",
         "config": dict(sizes, model=f"{model['name']} layer sizes, random weights", global_batch=batch, seq_len=context,
@@ -774,6 +779,10 @@ def main(argv=None):
                          "prefill, decode, --profile)")
     ap.add_argument("--design-size", default="", help="--design: which of the sizes (2k, 4k; commas between them; default all)")
     a = ap.parse_args(argv)
+    if a.quantize_head and not a.weight_bits:
+        ap.error("--quantize-head comes with --weight-bits")
+    if a.weight_bits and (a.design or a.impl == "reference"):            # a figure must not stand under the wrong form of the weights
+        ap.error("--weight-bits is for this engine's own workloads, not for --design or --impl reference")
     if a.warmup < 3:
         a.warmup = 3
     if a.gpus != 1:

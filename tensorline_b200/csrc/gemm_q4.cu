@@ -16,7 +16,8 @@
 // Every wait on a barrier is bounded: a block whose wait runs out records a code in `status`, stops and returns.
 #include "q4.cuh"
 
-int gemv_q4(Q4Args G, cudaStream_t stream);                        // gemv_q4.cu
+int gemv_q4_ranges(int tiles, int blocks, int sms);                // gemv_q4.cu
+int gemv_q4(Q4Args G, int splits, cudaStream_t stream);
 int gemm_q4_long(const Q4Args& G, int bn, cudaStream_t stream);     // gemm_q4_long.cu
 
 namespace {
@@ -305,13 +306,13 @@ struct QgPlan { int bn, long_, splits, first; double us; };      // tokens of a 
 // more 252), and clusters that find no room begin when others have ended.  Measured at 1, 2 .. 8 ranges, us:  45 tokens, 40 tiles x 108 blocks of k
 // 57 33 24 25 22 19 28 26;  64, 28 x 148: 77 44 31 25 27 24 23 20;  64, 216 x 40: 37 38 47 48 50 56;  128, 28 x 148: 70 44 32 25 41 36;
 // 128, 74 x 28: 18 19 28 33;  90, 16 x 32: 19 15 12 9.8 9.2 8.7.
-QgPlan qg_ranges(long long tiles, int blocks, int bn) {
-    const int sms = tl_num_sms(), two = bn <= 64;
+QgPlan qg_ranges(long long tiles, int blocks, int bn, int sms) {
+    const int two = bn <= 64;
     QgPlan p{bn, 0, 1, 0, 0};
     for (int s = 1; s <= 8 && s <= blocks; ++s) {
         const int per = (blocks + s - 1) / s;
         if ((blocks + per - 1) / per != s) continue;     // a range would be empty
-        const long long total = tiles * s, alone = s == 1 ? sms : s <= 3 ? sms * 9 / 10 : s == 4 ? sms * 4 / 5 : sms * 2 / 3;
+        const long long total = tiles * s, alone = s == 1 || sms == 1 ? sms : s <= 3 ? sms * 9 / 10 : s == 4 ? sms * 4 / 5 : sms * 2 / 3;
         const long long both = s == 1 ? 2 * sms : s <= 6 ? sms * 9 / 5 : sms * 17 / 10;
         const double turns = total <= alone ? 1 : two ? 1.4 * ((total + both - 1) / both) : (total + alone - 1) / alone;
         const double us = two ? turns * (per + 4) * (bn == 32 ? 0.5 : 0.6) + 2 : turns * (per * 0.44 + (s == 1 ? 5.5 : 9));
@@ -323,9 +324,9 @@ QgPlan qg_ranges(long long tiles, int blocks, int bn) {
 // One launch.  The blocks of gemm_q4_long.cu, one a SM, take a block of k through in 410, 420, 450 and 520 ns at 32, 64, 96 and 128 tokens: of its
 // tiles, the one with which they are done first.  Up to 64 tokens, and where there are so few tiles that many SMs would have none, ranges of K
 // in clusters are faster.  Measured, us, here / there:  128 tokens, 28 tiles x 148 blocks of k 25 / 65;  74 x 28 18 / 15.6;  256 tokens, 28 x 148 45 / 68.
-QgPlan qg_one(int T, int m_tiles, int blocks) {
-    const int here = T <= 32 ? 32 : T <= 64 ? 64 : 128, sms = tl_num_sms();
-    QgPlan p = qg_ranges((long long)m_tiles * ((T + here - 1) / here), blocks, here);
+QgPlan qg_one(int T, int m_tiles, int blocks, int sms) {
+    const int here = T <= 32 ? 32 : T <= 64 ? 64 : 128;
+    QgPlan p = qg_ranges((long long)m_tiles * ((T + here - 1) / here), blocks, here, sms);
     if (T > 64)
         for (int bn = 128; bn >= 32; bn -= 32) {
             const long long items = (long long)m_tiles * ((T + bn - 1) / bn), rounds = (items + sms - 1) / sms;
@@ -338,21 +339,30 @@ QgPlan qg_one(int T, int m_tiles, int blocks) {
 // Many tokens leave SMs idle in their last round of tiles, nearly all of them at worst: the tokens of that round may be better off by themselves, in
 // tiles of another size or in ranges of K.  Measured, us, at once / so:  2,048 tokens, 28 tiles of rows x 148 blocks of k (448 tiles, four more than
 // three rounds take) 340 / 275;  700 tokens 136 / 100;  1,500 tokens, 40 x 108 239 / 206;  2,048 tokens, 1,188 x 28 2,245 / 1,985.
-QgPlan qg_plan(int T, int m_tiles, int blocks) {
-    QgPlan p = qg_one(T, m_tiles, blocks);
+QgPlan qg_plan(int T, int m_tiles, int blocks, int sms) {
+    QgPlan p = qg_one(T, m_tiles, blocks, sms);
     for (int bn = 128; T > 128 && bn >= 64; bn -= 32) {
-        const int sms = tl_num_sms();
         const long long rounds = ((long long)m_tiles * ((T + bn - 1) / bn) + sms - 1) / sms - 1;      // full ones
         const long long first = rounds * sms / m_tiles * bn;
         if (first <= 0 || first >= T) continue;
-        const double us = (double)rounds * blocks * (0.37 + 0.0011 * bn) + 5 + qg_one(T - (int)first, m_tiles, blocks).us;
+        const double us = (double)rounds * blocks * (0.37 + 0.0011 * bn) + 5 + qg_one(T - (int)first, m_tiles, blocks, sms).us;
         if (us < p.us) p = QgPlan{bn, 1, 0, (int)first, us};
     }
     return p;
 }
 
-int qg_run(Q4Args G, const QgPlan& p, cudaStream_t stream) {
-    if (p.long_) return gemm_q4_long(G, p.bn, stream);
+// The next launch of a product of T tokens, and the tokens it takes.
+enum { QG_GEMV, QG_HERE, QG_LONG };
+struct QgLaunch { int tokens, kernel, bn, splits; };
+QgLaunch qg_next(int T, int m_tiles, int blocks, int sms) {
+    if (T <= Q4_FEW) return QgLaunch{T, QG_GEMV, T <= 8 ? 8 : 16, gemv_q4_ranges(m_tiles, blocks, sms)};
+    const QgPlan p = qg_plan(T, m_tiles, blocks, sms);
+    return QgLaunch{p.first ? p.first : T, p.long_ ? QG_LONG : QG_HERE, p.bn, p.long_ ? 1 : p.splits};
+}
+
+int qg_run(Q4Args G, const QgLaunch& p, cudaStream_t stream) {
+    if (p.kernel == QG_GEMV) return gemv_q4(G, p.splits, stream);
+    if (p.kernel == QG_LONG) return gemm_q4_long(G, p.bn, stream);
     const int tiles = (G.N + Q4_ROWS - 1) / Q4_ROWS;
     G.per = (G.blocks + p.splits - 1) / p.splits;
     CUtensorMap map;
@@ -391,16 +401,28 @@ TL_EXPORT int tl_gemm_q4(const void* x, long long ldx, const void* w, void* y, l
     G.x = (const unsigned char*)x; G.ldx = ldx; G.w = (const unsigned char*)w; G.blocks = (K + Q4_K - 1) / Q4_K;
     G.out = y; G.out_f32 = out_f32; G.ldo = ldo; G.N = N; G.K = K; G.T = T;
     G.gate = gate; G.limit = limit; G.alpha = alpha; G.at_rest = at_rest; G.status = status;
-    const int m_tiles = (N + Q4_ROWS - 1) / Q4_ROWS;
-    while (G.T > Q4_FEW) {
-        const QgPlan p = qg_plan(G.T, m_tiles, G.blocks);
-        if (!p.first) return qg_run(G, p, stream);
-        const int rest = G.T - p.first;
-        G.T = p.first;
+    const int m_tiles = (N + Q4_ROWS - 1) / Q4_ROWS, sms = tl_num_sms();
+    for (int left = T; left > 0;) {
+        const QgLaunch p = qg_next(left, m_tiles, G.blocks, sms);
+        G.T = p.tokens;
         if ((e = qg_run(G, p, stream))) return e;
-        G.T = rest;
-        G.x += (size_t)p.first * G.ldx * 2;
-        G.out = (unsigned char*)G.out + (size_t)p.first * G.ldo * (out_f32 ? 4 : 2);
+        left -= p.tokens;
+        G.x += (size_t)p.tokens * G.ldx * 2;
+        G.out = (unsigned char*)G.out + (size_t)p.tokens * G.ldo * (out_f32 ? 4 : 2);
     }
-    return gemv_q4(G, stream);
+    return 0;
+}
+
+// The launches that `tl_gemm_q4` makes of a product of T tokens with N x K weights on `sms` SMs: their number, 0 for sizes that it does not take.  The
+// first `room` of them to `launches`, four ints each: its tokens, its kernel (0 gemv_q4.cu, 1 this file's, 2 gemm_q4_long.cu), the
+// tokens of a tile, the ranges of K.
+TL_EXPORT int tl_gemm_q4_plan(int T, int N, int K, int sms, int* launches, int room) {
+    if (T < 1 || T > Q4_MOST || N < 1 || N > Q4_MOST || K < 1 || K > Q4_MOST || (K & 7) || sms < 1) return 0;
+    int n = 0;
+    for (int left = T; left > 0; ++n) {
+        const QgLaunch p = qg_next(left, (N + Q4_ROWS - 1) / Q4_ROWS, (K + Q4_K - 1) / Q4_K, sms);
+        if (n < room) { launches[4 * n] = p.tokens; launches[4 * n + 1] = p.kernel; launches[4 * n + 2] = p.bn; launches[4 * n + 3] = p.splits; }
+        left -= p.tokens;
+    }
+    return n;
 }

@@ -195,13 +195,14 @@ int gv_launch_form(const CUtensorMap& map, const Q4Args& G, int tiles, int split
            G.form.group == 64 ? gv_launch<NT, 64, false>(map, G, tiles, splits, stream) : gv_launch<NT, 32, false>(map, G, tiles, splits, stream);
 }
 
+}  // namespace
+
 // Ranges of K a tile: the fewest blocks of k, one behind the other, on the SM that has most.  An SM gets through a block of k in the same time
 // whether one thread block works on it or two do, so with more of them than SMs every SM counts twice; clusters of many blocks leave some SMs
 // of a GPC empty (of 148 SMs about 132 get a block in clusters of two or three, 100 in larger ones, where two blocks go to one SM first).  Measured
 // at 1, 2 .. 8 ranges, us:  28 tiles x 148 blocks 45 24 17.5 17 17 16 14.7 13.6;  40 x 108: 33 18 13.2 16 14.5 13.3 17 16;  36 x 28: 9.7 6.2
 // 5.6 6.0 5.4 6.2 6.2 6.2;  86 x 16: 6.4 7.2 7.8 6.9 7.0 9.5 9.3 9.1;  296 x 28: 17 21 27 29 27 29 32 32.
-int gv_ranges(int tiles, int blocks) {
-    const int sms = tl_num_sms();
+int gemv_q4_ranges(int tiles, int blocks, int sms) {
     int best = 1;
     long long least = 0;
     for (int s = 1; s <= 8 && s <= blocks; ++s) {
@@ -215,11 +216,9 @@ int gv_ranges(int tiles, int blocks) {
     return best;
 }
 
-}  // namespace
-
 // The product for G.T <= Q4_FEW tokens; `G` is filled in but for the ranges of K and the ring (gemm_q4.cu).
-int gemv_q4(Q4Args G, cudaStream_t stream) {
-    const int tiles = (G.N + Q4_ROWS - 1) / Q4_ROWS, splits = gv_ranges(tiles, G.blocks);
+int gemv_q4(Q4Args G, int splits, cudaStream_t stream) {
+    const int tiles = (G.N + Q4_ROWS - 1) / Q4_ROWS;
     G.per = (G.blocks + splits - 1) / splits;
     CUtensorMap map;
     int e = load_encode();

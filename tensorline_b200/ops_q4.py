@@ -15,12 +15,13 @@ Launches go to the current stream of the tensors' device.  As with every matrix 
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 
 from . import ops
 from .csrc.build import load_library
-from .ops import KernelError, _check, _stream, device_status
+from .ops import KernelError, _check, _stream, device_status, num_sms
 
 _P, _I, _F, _L = ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_longlong
 
@@ -28,6 +29,7 @@ SOURCES = ["gemm_q4.cu", "gemm_q4_long.cu", "gemv_q4.cu", "quantize_q4.cu"]
 _SIGNATURES = {
     "tl_q4_block_bytes": [_I, _I, _I],
     "tl_gemm_q4": [_P, _L, _P, _P, _L, _I, _I, _I, _I, _F, _F, _P, _P],
+    "tl_gemm_q4_plan": [_I, _I, _I, _I, _P, _I],
     "tl_quantize_q4": [_P, _I, _P, _I, _I, _I, _P],
     "tl_dequantize_q4": [_P, _P, _I, _I, _I, _I, _P],
 }
@@ -194,6 +196,22 @@ def pack(codes: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor | None =
     return Q4Weight(data, n, k, group, zeros is not None, scales.dtype)
 
 
+KERNELS = ("gemv_q4", "gemm_q4", "gemm_q4_long")
+
+
+def plan(T: int, n: int, k: int, sms: int) -> list:
+    """The launches of a product of T tokens with a matrix [n, k] on a GPU of `sms` SMs: (tokens, kernel, tokens of a tile, ranges of K)."""
+    count = lib().tl_gemm_q4_plan(T, n, k, sms, None, 0)
+    room = (ctypes.c_int * (4 * count))()
+    lib().tl_gemm_q4_plan(T, n, k, sms, room, count)
+    return [(room[4 * i], KERNELS[room[4 * i + 1]], room[4 * i + 2], room[4 * i + 3]) for i in range(count)]
+
+
+@functools.lru_cache(maxsize=4096)
+def _launches(T: int, n: int, k: int, index: int) -> int:
+    return lib().tl_gemm_q4_plan(T, n, k, num_sms(torch.device("cuda", index)), None, 0)
+
+
 _GATES = {"silu": 1 << 10, "gelu_tanh": 2 << 10, True: 1 << 10}
 _OUT_F32, _AT_REST = 1 << 12, 1 << 13
 _status: dict = {}                                        # device index -> address of its status word
@@ -275,7 +293,8 @@ def gemm_q4(x: torch.Tensor, w: Q4Weight, out_dtype: torch.dtype = torch.bfloat1
     if status is None:
         status = _status[index] = device_status(x.device).data_ptr()
     _check((_lib or lib()).tl_gemm_q4(ptr, ldx, data.data_ptr(), out.data_ptr(), ldo, T, n, k, form, limit, alpha, status,
-                                      torch._C._cuda_getCurrentRawStream(index)), "gemm_q4+gated" if gated else "gemm_q4")
+                                      torch._C._cuda_getCurrentRawStream(index)), "gemm_q4+gated" if gated else "gemm_q4",
+           launches=1 if T <= 128 else _launches(T, n, k, index))       # (up to 128 tokens are never cut)
     return out
 
 

@@ -1,0 +1,26 @@
+"""How products with weights of 4 bits are cut into launches (no GPU: the plan is the host's)."""
+import pytest
+
+from tensorline_b200 import ops_q4
+
+SIZES = [(t, n, k) for t in (1, 8, 9, 16, 17, 32, 33, 64, 65, 100, 128, 129, 333, 512, 643, 700, 1284, 2048, 2049, 5000, 100_000)
+         for n, k in ((1, 8), (128, 128), (640, 8192), (3584, 18944), (37888, 3584), (152064, 3584), (300, 1_000_000))]
+
+
+@pytest.mark.parametrize("sms", [148, 132, 2, 1])
+def test_every_token_is_taken_once_and_every_range_holds_something(sms):
+    for T, n, k in SIZES:
+        launches = ops_q4.plan(T, n, k, sms)
+        blocks = -(-k // 128)
+        assert sum(tokens for tokens, *_ in launches) == T and all(tokens > 0 for tokens, *_ in launches)
+        assert len(launches) == 1 or T > 128             # what `gemm_q4` counts on
+        for tokens, kernel, tile, ranges in launches:
+            assert 1 <= ranges <= 8 and -(-blocks // -(-blocks // ranges)) == ranges
+            assert tile in {"gemv_q4": (8, 16), "gemm_q4": (32, 64, 128), "gemm_q4_long": (32, 64, 96, 128)}[kernel]
+            assert (kernel == "gemv_q4") == (tokens <= 16) and (kernel != "gemv_q4" or tokens <= tile) and (kernel != "gemm_q4_long" or ranges == 1)
+
+
+def test_sizes_that_no_product_has():
+    lib = ops_q4.lib()
+    for T, n, k, sms in ((0, 128, 64, 148), (1, 0, 64, 148), (1, 128, 60, 148), (1, 128, 64, 0), (0x7fffff01, 128, 64, 148)):
+        assert lib.tl_gemm_q4_plan(T, n, k, sms, None, 0) == 0

@@ -22,7 +22,7 @@ int gemm_q4_long(const Q4Args& G, int bn, cudaStream_t stream);     // gemm_q4_l
 
 namespace {
 
-constexpr int QG_STAGES_MAX = 12;
+constexpr int QG_STAGES_MAX = 12, QG_TILES_MOST = 65535;           // tiles of tokens: a grid's second dimension
 
 template <int BN> struct QgShape {
     static constexpr int X_HALF = BN * 128, X_BYTES = 2 * X_HALF;         // BN tokens x 64 k, twice
@@ -331,7 +331,7 @@ QgPlan qg_one(int T, int m_tiles, int blocks, int sms) {
         for (int bn = 128; bn >= 32; bn -= 32) {
             const long long items = (long long)m_tiles * ((T + bn - 1) / bn), rounds = (items + sms - 1) / sms;
             const double us = (double)rounds * blocks * (0.37 + 0.0011 * bn) + 3;
-            if (us < p.us) p = QgPlan{bn, 1, 0, 0, us};
+            if (us < p.us || (!p.long_ && (T + here - 1) / here > QG_TILES_MOST)) p = QgPlan{bn, 1, 0, 0, us};
         }
     return p;
 }

@@ -24,3 +24,11 @@ def test_sizes_that_no_product_has():
     lib = ops_q4.lib()
     for T, n, k, sms in ((0, 128, 64, 148), (1, 0, 64, 148), (1, 128, 60, 148), (1, 128, 64, 0), (0x7fffff01, 128, 64, 148)):
         assert lib.tl_gemm_q4_plan(T, n, k, sms, None, 0) == 0
+
+
+@pytest.mark.parametrize("T", [65535 * 128, 65535 * 128 + 1, 9_000_000, 0x7fffff00])
+@pytest.mark.parametrize("n,k", [(8, 10_000), (8, 20_000), (1, 200_000), (128, 8)])
+def test_grids_that_a_launch_can_have(T, n, k):
+    """Tiles of tokens are the grid's second dimension in `gemm_q4`, which ends at 65,535; `gemm_q4_long` has one block an SM."""
+    for tokens, kernel, tile, _ in ops_q4.plan(T, n, k, 148):
+        assert kernel != "gemm_q4" or -(-tokens // tile) <= 65535

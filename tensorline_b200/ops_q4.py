@@ -238,6 +238,12 @@ def _meet(a: int, a_step: int, a_bytes: int, b: int, b_step: int, b_bytes: int, 
     return True
 
 
+def _reach(a: int, step: int, wide: int, rows: int, b: int, size: int) -> bool:
+    """Whether one of `rows` rows of `wide` bytes, `step` bytes from row to row, from address a on, has a byte of the `size` at b."""
+    r = max(0, (b - wide - a) // step + 1)               # the first row that ends behind b
+    return r < rows and a + r * step < b + size
+
+
 # A call takes the host 7 us and the smallest products 5 us, so what is asked of a tensor is asked once, and nothing is built that the call does
 # not need (10.5 us with properties of the device and an argument for each of the weights' properties).
 def gemm_q4(x: torch.Tensor, w: Q4Weight, out_dtype: torch.dtype = torch.bfloat16, *, gated=False, out: torch.Tensor | None = None) -> torch.Tensor:
@@ -245,7 +251,7 @@ def gemm_q4(x: torch.Tensor, w: Q4Weight, out_dtype: torch.dtype = torch.bfloat1
     Rows of x may lie apart (a multiple of 8 values); T may be 0.
     `gated` ("silu", "gelu_tanh" or ("swish_clamped", limit, alpha)): w holds gate and up rows alternating in blocks of 64 (N a multiple of
     128), the result is act(gate) * up, [T, N / 2], from the float32 sums.  `out`: a tensor to write, of the result's shape and type, with rows
-    that may lie apart, that shares no memory with x."""
+    that may lie apart, that shares no memory with x or w."""
     n, k, data = w.n, w.k, w.data
     form, limit, alpha = w.form, 0.0, 1.0
     if gated:
@@ -284,6 +290,8 @@ def gemm_q4(x: torch.Tensor, w: Q4Weight, out_dtype: torch.dtype = torch.bfloat1
         _device(x, out)
         if _meet(ptr, ldx * 2, k * 2, out.data_ptr(), ldo * out_dtype.itemsize, cols * out_dtype.itemsize, T):
             raise KernelError("gemm_q4: out shares memory with x")
+        if _reach(out.data_ptr(), ldo * out_dtype.itemsize, cols * out_dtype.itemsize, T, data.data_ptr(), data.numel()):
+            raise KernelError("gemm_q4: out shares memory with the weights")
     if T == 0:
         return out
     if index != torch._C._cuda_getDevice():

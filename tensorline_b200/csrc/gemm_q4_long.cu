@@ -305,6 +305,13 @@ gemm_q4_long_kernel(const __grid_constant__ CUtensorMap map_x, const QlArgs A) {
 template <int GROUP, bool ZEROS>
 int ql_launch(const CUtensorMap& map, const QlArgs& A, int blocks, cudaStream_t stream) {
     static bool raised[TL_MAX_DEVICES] = {};
+    const int dev = tl_device_index();
+    if (dev >= 0 && !raised[dev]) {                      // the shares are of what this build's blocks are launched with
+        cudaFuncAttributes a;
+        const cudaError_t ce = cudaFuncGetAttributes(&a, gemm_q4_long_kernel<GROUP, ZEROS>);
+        if (ce != cudaSuccess) return (int)ce;
+        if (5 * ((a.numRegs + 7) & ~7) < QL_REGS_COPY + 2 * QL_REGS_UNPACK + 2 * QL_REGS_SUM) return (int)cudaErrorLaunchOutOfResources;
+    }
     const int e = tl_raise_smem(gemm_q4_long_kernel<GROUP, ZEROS>, raised, QL_SMEM);
     if (e) return e;
     return launch_after_wait(gemm_q4_long_kernel<GROUP, ZEROS>, dim3(blocks), dim3(QL_THREADS), QL_SMEM, stream, map, A);

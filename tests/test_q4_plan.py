@@ -1,7 +1,11 @@
 """How products with weights of 4 bits are cut into launches (no GPU: the plan is the host's)."""
+import math
+import random
+
 import pytest
 
 from tensorline_b200 import ops_q4
+from tests.q4_shapes import SHAPES, SMS, ways
 
 SIZES = [(t, n, k) for t in (1, 8, 9, 16, 17, 32, 33, 64, 65, 100, 128, 129, 333, 512, 643, 700, 1284, 2048, 2049, 5000, 100_000)
          for n, k in ((1, 8), (128, 128), (640, 8192), (3584, 18944), (37888, 3584), (152064, 3584), (300, 1_000_000))]
@@ -32,3 +36,19 @@ def test_grids_that_a_launch_can_have(T, n, k):
     """Tiles of tokens are the grid's second dimension in `gemm_q4`, which ends at 65,535; `gemm_q4_long` has one block an SM."""
     for tokens, kernel, tile, _ in ops_q4.plan(T, n, k, 148):
         assert kernel != "gemm_q4" or -(-tokens // tile) <= 65535
+
+
+def test_the_tested_shapes_take_every_way_that_there_is():
+    """Sizes all over the range, drawn: what a plan does with one of them is in `test_q4_shapes_gpu.py`, plain and gated, whatever the prices are changed to."""
+    rng = random.Random(5)
+    log = lambda lo, hi: int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))    # noqa: E731
+    seen = set()
+    for _ in range(20_000):
+        n, k = log(1, 160_000), 8 * log(1, 4000)
+        seen |= ways(ops_q4.plan(log(1, 5000), n, k, SMS), n)
+    for kind in (1, 2):
+        tested = set().union(*(ways(ops_q4.plan(shape[0], shape[kind], shape[3], SMS), shape[kind]) for shape in SHAPES))
+        assert seen <= tested, sorted(seen - tested)
+    assert {tile for kernel, tile, _ in seen if kernel == "gemm_q4"} == {32, 64, 128} and {tile for kernel, tile, _ in seen if kernel == "gemm_q4_long"} >= {64, 96, 128}
+    ranges = {r for T, n, _, k in SHAPES for _, kernel, tile, r in ops_q4.plan(T, n, k, SMS) if (kernel, tile) == ("gemm_q4", 128)}
+    assert ranges >= {1, 2, 3, 4, 6, 7, 8}

@@ -140,16 +140,6 @@ gemm_q4_kernel(const __grid_constant__ CUtensorMap map_x, const Q4Args G) {
             if (!ok) break;
             if (++s == S) s = 0;
         }
-        // Tensor memory goes back as soon as the sums have left it, before anyone waits for the cluster: a block that holds columns waits for its own
-        // copies only.  (On two streams this kernel's clusters and a product in pairs, which takes all columns of two SMs, could each hold what the other waits for.)
-        asm volatile("bar.sync 1, %0;" ::"n"(32 * (SUMS + 1)) : "memory");
-        if (*abort_flag) {                               // products in flight end first
-            const long long begin = clock64();
-            while (clock64() - begin < 2000000LL) { }
-        }
-        __syncwarp();
-        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(Sh::COLS) : "memory");
     } else if (warp < 6) {
         // ---------------------------------------------------------------- unpacking
         const int row = quarter * 32 + lane, zeros_at = Q4_CODES + G.form.groups * Q4_ROWS * (G.form.scale_f32 ? 4 : 2);
@@ -247,6 +237,18 @@ gemm_q4_kernel(const __grid_constant__ CUtensorMap map_x, const Q4Args G) {
 #pragma unroll
             for (int c = 0; c < CW; ++c) red[(part * CW + c) * Q4_ROWS + row] = acc[c];
         }
+    }
+    // Tensor memory goes back as soon as the sums have left it, before anyone waits for the cluster: a block that holds columns waits for its own copies
+    // only.  (On two streams this kernel's clusters and a product in pairs, which takes all columns of two SMs, could each hold what the other waits for.)
+    if (warp == 1) {
+        asm volatile("bar.sync 1, %0;" ::"n"(32 * (SUMS + 1)) : "memory");
+        if (*abort_flag) {                               // products in flight end first
+            const long long begin = clock64();
+            while (clock64() - begin < 2000000LL) { }
+        }
+        __syncwarp();
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(Sh::COLS) : "memory");
     }
     if (nz > 1 || G.gate) {
         if (nz > 1) pair_cluster_sync(); else __syncthreads();

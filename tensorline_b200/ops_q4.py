@@ -300,9 +300,11 @@ def gemm_q4(x: torch.Tensor, w: Q4Weight, out_dtype: torch.dtype = torch.bfloat1
     status = _status.get(index)
     if status is None:
         status = _status[index] = device_status(x.device).data_ptr()
-    _check((_lib or lib()).tl_gemm_q4(ptr, ldx, data.data_ptr(), out.data_ptr(), ldo, T, n, k, form, limit, alpha, status,
-                                      torch._C._cuda_getCurrentRawStream(index)), "gemm_q4+gated" if gated else "gemm_q4",
-           launches=1 if T <= 128 else _launches(T, n, k, index))       # (up to 128 tokens are never cut)
+    code = (_lib or lib()).tl_gemm_q4(ptr, ldx, data.data_ptr(), out.data_ptr(), ldo, T, n, k, form, limit, alpha, status, torch._C._cuda_getCurrentRawStream(index))
+    if T <= 128:                                         # never cut
+        _check(code, "gemm_q4+gated" if gated else "gemm_q4")
+    else:
+        _check(code, "gemm_q4+gated" if gated else "gemm_q4", _launches(T, n, k, index))
     return out
 
 

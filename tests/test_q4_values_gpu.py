@@ -1,7 +1,7 @@
 """Decoders with weights of 4 bits beside the same decoders with the values that those weights stand for, quantized by the plain code and stored in 32 bits.
 
 The 32-bit engine reads the values exactly, so its logits are the same bits either way.  The bfloat16 engine is held against them by the rule that the decoders
-without experts have for weights of 16 bits: every position within 0.05 of the request's largest logit."""
+without experts have for weights of 16 bits, every position within 0.05 of the largest logit, and by that of the others, four positions in five."""
 import importlib
 import json
 
@@ -75,9 +75,11 @@ def test_the_logits_of_the_values(tmp_path, monkeypatch, decoder, name):
     assert bool(given) == bool(names) and (not given or ("head" in names) == own_head)    # widths that are no multiple of 8 stay as they are
     want = logits(Engine(str(values), dtype="float32", block_size=page, **OPTIONS), vocab)
     assert torch.equal(exact, want)
+    err = (logits(Engine(str(folder), dtype="bfloat16", **bits), vocab) - want).abs().amax(1) / want.abs().max()
     if decoder in ("zosurax", "fimolix"):
-        err = (logits(Engine(str(folder), dtype="bfloat16", **bits), vocab) - want).abs().amax(1)
-        assert float(err.max()) <= 0.05 * float(want.abs().max()), (err / want.abs().max()).tolist()
+        assert float(err.max()) <= 0.05, err.tolist()
+    else:                                                # a position's experts may change with a rounding
+        assert float(err.max()) <= 1.0 and int((err > 0.05).sum()) <= 0.2 * len(err), err.tolist()
 
 
 @pytest.mark.parametrize("name,group,zeros,head", [("A", 64, True, False), ("B_FULL", 32, False, True), ("B", 32, True, True), ("C", 128, False, False)])

@@ -35,7 +35,8 @@ def _generate_parser() -> argparse.ArgumentParser:
     ap.add_argument("--block-size", type=int, default=16)
     ap.add_argument("--num-blocks", type=int, default=None, help="KV pages (default: fit 60%% of free memory)")
     ap.add_argument("--kv-cache-gb", type=float, default=None, help="KV cache size (default: 60%% of free memory)")
-    ap.add_argument("--weight-bits", type=int, choices=[4], default=None, help="quantize the layers' matrices to 4 bits as they are loaded")
+    ap.add_argument("--weight-bits", type=int, choices=[4], default=None, help="quantize the layers' matrices (not routed experts) to 4 bits as they are loaded: "
+                    "faster steps of few tokens, slower prompts")
     ap.add_argument("--weight-group", type=int, choices=[32, 64, 128], default=128, help="values that share a scale (with --weight-bits)")
     ap.add_argument("--weight-zeros", action="store_true", help="a zero point beside every scale (with --weight-bits)")
     ap.add_argument("--quantize-head", action="store_true", help="the output head in 4 bits too (with --weight-bits)")

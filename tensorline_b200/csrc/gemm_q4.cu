@@ -11,8 +11,8 @@
 // tensor memory, scale and add them in registers.  Weights in tensor memory cost one store of 32 values a warp instead of a swizzled round
 // trip through shared memory, and their scale is one number a thread, since a row is a lane.
 // What bounds it: hand-overs between those warps, 540 ns a block of k at 64 tokens and 1.4 times that for two thread blocks an SM (unpacking alone 230,
-// the weights' way from memory 190).  Measured in a CUDA graph: 37,888 x 3,584 gated, 32 tokens 23 us, 64 tokens 29 us (floor 10.7); 3,584 x
-// 18,944, 64 tokens 20 us (5.3); 5,120 x 13,824 in groups of 64 with zeros and float scales, 45 tokens 23.5 us (6.4).
+// the weights' way from memory 190).  Measured in a CUDA graph on weights that are not in L2: 37,888 x 3,584 gated, 32 tokens 22.7 us, 64 tokens 29.4 us
+// (floor 10.7); 3,584 x 18,944, 64 tokens 20 us (5.8), 128 tokens 24.8 (10.7); 5,120 x 13,824 in groups of 64 with zeros and float scales, 45 tokens 23.5 us (6.4).
 // Every wait on a barrier is bounded: a block whose wait runs out records a code in `status`, stops and returns.
 #include "q4.cuh"
 

@@ -4,10 +4,10 @@
 // row a thread), one warp issues eight products of 16 k a block, eight warps scale a finished group's sums and add them to the outputs', which
 // they hold in registers, 64 a thread at most.  Tensor memory: four blocks of unpacked weights (64 columns each) and two groups' sums (2 x 128),
 // all of it.  The ring of copies and the buffers run on from one tile to the next.
-// What bounds it: a block of k takes 1,000 cycles at 128 tokens, of which the tensor cores need 520; the summing warps are never idle (125 cycles a wait
-// for the products, of which 80 however long ago they were over, twice 200 for a load of 32 columns from tensor memory and 125 for their
-// multiply-adds, which share their pipe with the unpacking, 70 for two arrivals).  Measured in a CUDA graph, 37,888 x 3,584 gated: 96 tokens 36 us
-// (floor 16), 2,048 tokens 600 to 640 us (floor 341: 0.9 PFLOP/s); 7,168 x 5,120, 333 tokens: 42 us (15).
+// What bounds it: the summing warps' chain.  A block of k takes 1,000 cycles at 128 tokens, of which the tensor cores need 520; the summing warps have one thing
+// to do behind the other, most of it waiting (125 cycles for the products, of which 80 however long ago they were over, twice 200 for a load of
+// 32 columns from tensor memory; 125 for their multiply-adds, which share their pipe with the unpacking, 70 for two arrivals).  Measured in a CUDA
+// graph, 37,888 x 3,584 gated: 96 tokens 35 us (floor 16), 2,048 tokens 631 to 651 us (floor 341: 0.86 PFLOP/s); 7,168 x 5,120, 333 tokens: 42 us (15).
 // Not faster: pairs of blocks on 256 rows and 192 tokens (half as many bytes of tokens; they hand over through the cluster, about 500 cycles a time,
 // with no tensor memory left to hide it: 1,250 cycles a block of k and 5 a token), sixteen summing warps of 32 tokens (2 % slower: 80 registers
 // are too few), tokens and weights in rings of their own (7 %: one commit more), two warps that issue products, more warps that unpack.

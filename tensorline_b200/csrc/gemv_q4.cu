@@ -7,9 +7,13 @@
 // cycle and SM a block of 128 x 128 weights has to be through in about 370 cycles, and its hand-overs to and from tcgen05 (an arrival, a
 // wait and a commit each) took longer.  The order of k within a product is free, so a lane takes eight k that follow one another from one word
 // of codes and from one 16-byte piece of a token.
-// What bounds it: the weights' bytes, and nearly as much their unpacking, 11 instructions for eight values on two pipes, 440 cycles a block of 128 x 128
-// with the products.  Measured in a CUDA graph, 37,888 x 3,584 gated (70 MB): 1 token 16.9 us, 8 tokens 17.9, 16 tokens 21.4 (floor 10.7: 4.2 of
-// 6.5 TB/s); 152,064 x 3,584 with zeros, 8 tokens 72 us (44); 4,608 x 3,584, 1 token 5.7 us (1.3: half of it begins and ends a launch).
+// What bounds it: latency with few warps.  No pipe is full (8 tokens, a cold launch: a scheduler issues in 49 % of the cycles, the ALU, which takes seven of the
+// 11 instructions for eight values, is used in 43 %): a scheduler has four working warps, and between two instructions of one lie 8.1 cycles, of
+// which it waits 1.8 for copies and loads, 1.1 for the instruction before, 1.0 for a pipe and 1.3 for its turn.  A block of 128 x 128 takes 440 cycles so, where
+// memory needs 370; beside that whole tiles are dealt out (1,188 tiles on 296 places are four rounds and four tiles more), and every tile begins and ends anew.
+// Measured in a CUDA graph on weights that are not in L2, 37,888 x 3,584 gated (70 MB): 1 token 16.8 us, 8 tokens 17.3, 16 tokens 21.0 (floor 10.7: 4.1
+// of 6.5 TB/s); 152,064 x 3,584 with zeros, 8 tokens 71 us (44); 3,584 x 18,944, 8 tokens 13.7 us (5.4); 4,608 x 3,584, 1 token 5.6 us (1.3: half of
+// it begins and ends a launch).
 #include "q4.cuh"
 
 namespace {

@@ -425,7 +425,7 @@ TL_EXPORT int tl_gemm_q4(const void* x, long long ldx, const void* w, void* y, l
 // first `room` of them to `launches`, four ints each: its tokens, its kernel (0 gemv_q4.cu, 1 this file's, 2 gemm_q4_long.cu), the
 // tokens of a tile, the ranges of K.
 TL_EXPORT int tl_gemm_q4_plan(int T, int N, int K, int sms, int* launches, int room) {
-    if (T < 1 || T > Q4_MOST || N < 1 || N > Q4_MOST || K < 1 || K > Q4_MOST || (K & 7) || sms < 1) return 0;
+    if (T < 1 || T > Q4_MOST || N < 1 || N > Q4_MOST || K < 1 || K > Q4_MOST || (K & 7) || sms < 1 || (room > 0 && !launches)) return 0;
     int n = 0;
     for (int left = T; left > 0; ++n) {
         const QgLaunch p = qg_next(left, (N + Q4_ROWS - 1) / Q4_ROWS, (K + Q4_K - 1) / Q4_K, sms);

@@ -308,4 +308,4 @@ def gemm_q4(x: torch.Tensor, w: Q4Weight, out_dtype: torch.dtype = torch.bfloat1
     return out
 
 
-__all__ = ["Q4Weight", "block_bytes", "dequantize", "gemm_q4", "pack", "quantize", "lib"]
+__all__ = ["Q4Weight", "block_bytes", "dequantize", "gemm_q4", "pack", "plan", "quantize", "lib"]

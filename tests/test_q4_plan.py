@@ -28,6 +28,7 @@ def test_sizes_that_no_product_has():
     lib = ops_q4.lib()
     for T, n, k, sms in ((0, 128, 64, 148), (1, 0, 64, 148), (1, 128, 60, 148), (1, 128, 64, 0), (0x7fffff01, 128, 64, 148)):
         assert lib.tl_gemm_q4_plan(T, n, k, sms, None, 0) == 0
+    assert lib.tl_gemm_q4_plan(700, 3584, 4096, 148, None, 0) == 2 and lib.tl_gemm_q4_plan(700, 3584, 4096, 148, None, 2) == 0      # nowhere to write them
 
 
 @pytest.mark.parametrize("T", [65535 * 128, 65535 * 128 + 1, 9_000_000, 0x7fffff00])
